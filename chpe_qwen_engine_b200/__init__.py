@@ -81,6 +81,13 @@ SYMBOLS = [
     ("chpe_kv_page_table", _I, [_P, _U32P, _U32, _U32P]),
     ("chpe_probe_gemv_linear", _I, [_P, _U64, _U64, _FP, _U64, _FP, _U64, _U64, _I, _I64]),
     ("chpe_attention_decode_noalloc", _I, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _F, _P]),
+    ("chpe_qk_norm_rope", _I, [_P, _P, _P, _I, _I64, _I64, _I64, _U32, _U32, _U32, _U32, _P, _P, _F, _F, _P, _P,
+                               _U32, _P, _I64, _P, _I64, _P, _P, _I, _U64, _P, _P]),
+    ("chpe_attention_decode_paged_workspace", _S, [_U32]),
+    ("chpe_attention_decode_paged", _I, [_P, _I, _I64, _P, _P, _I, _U32, _U32, _P, _I64, _U32, _P, _U32, _U32, _U32, _U32,
+                                         _F, _P, _I64, _P, _P, _S, _P]),
+    ("chpe_logits_process", _I, [_P, _I, _I64, _U32, _U32, _P, _I64, _U32, _P, _P, _P, _P, _P, _P, _P, _I64, _U32,
+                                 _P, _I64, _P, _I64, _P, _P]),
     ("chpe_probe_attention", _I, [_P, _U32, _U32, _FP, _FP, _FP, _FP]),
     ("chpe_probe_embed", _I, [_P, _U32, _FP]),
     ("chpe_probe_wait_timeout", _I, [_P, _U32]),

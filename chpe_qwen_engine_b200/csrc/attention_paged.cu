@@ -1,0 +1,631 @@
+// attention_paged.cu -- decode attention of a batch of sequences over a paged
+// K/V cache: one new token per sequence, page tables and lengths on the device.
+//
+//   out[b,h] = sum_t p[t] v[t],  p = softmax over t < len[b] of scale * q[b,h].k[t]
+//   lse[b,h] = log sum_t exp(scale * q[b,h].k[t])
+//
+// with position t of sequence b in row t % page of page table[b][t / page].
+// Query heads h*G .. h*G+G-1 share kv head h.  Bound by memory: every K and V
+// row is read once, 4*H/KV flops for each 2 elements.
+//
+// Work split.  The work is a line of tiles of 64 positions: sequence by
+// sequence, head by head, tile by tile.  CTA c of C takes the c-th of C equal
+// stretches, whatever sequences lie in it, so a batch of very different
+// lengths, one long sequence and many short ones all fill the GPU alike and
+// the host never learns a length (a captured graph stays valid as sequences
+// grow).  A (sequence, head) that lies in one CTA is finished there; of one
+// cut between CTAs each writes a partial record (values, maximum, sum) and
+// combine_kernel, launched behind with programmatic dependent launch, joins the records in
+// the order of the positions: results do not depend on timing.
+//
+// Inside a CTA the four warps take the four 16-position units of a tile, each
+// with a ring of its own in shared memory (cp.async, 16-byte chunks XOR-swizzled
+// by row so that ldmatrix is free of bank conflicts) and a running maximum of
+// its own; they meet once per stretch.
+//
+// Matrix instructions: mma.sync m16n8k16.  A batch-1 product has 8 query heads
+// at most per tile against 16 rows of the instruction; the spare 8 rows carry the low
+// halves: q is split into hi + lo of the cache's type (rows 0-7 and 8-15), and
+// so is the probability, so products keep 16 (BF16) or 22 (FP16) bits at no
+// cost.  Float queries over a BF16 cache take a second pass with a third part.
+// tcgen05.mma would need its 128-row operand in shared memory or TMEM for 8 rows
+// of work; the tensor pipe is nearly idle here either way.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "device_common.cuh"
+#include "serve_common.h"
+
+namespace {
+
+constexpr int kWarps = 4, kUnit = 16, kTile = kWarps * kUnit;
+constexpr int kHeads = 8;          // query heads of one tile (a "virtual" kv head)
+constexpr int kMaxCtas = 512;      // grid limit, sizes the workspace
+constexpr float kPShift = 14.f;    // probabilities are held times 2^14: FP16 keeps small ones
+
+struct PagedLaunch {
+  const void* q;
+  int32_t q_type;
+  int64_t q_stride;
+  const void *kc, *vc;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  uint32_t n_pages, page_shift;
+  int64_t cap;  // positions a table row can hold
+  int32_t B, H, KV, G, HT, VH;  // VH = KV * HT virtual heads of up to 8 query heads
+  float scale;
+  void* out;
+  int64_t out_stride;
+  float* lse;
+  float* part;  // [2 * grid][8][D + 2]
+  int4* desc;   // [grid]: sequence, virtual head, number of records, unused
+};
+
+template <typename T>
+CHPE_DEV uint32_t pack2(float a, float b);
+template <>
+CHPE_DEV uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+CHPE_DEV uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+CHPE_DEV float2 unpack2(uint32_t w);
+template <>
+CHPE_DEV float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+CHPE_DEV float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
+template <typename T>
+CHPE_DEV void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+CHPE_DEV void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+CHPE_DEV void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+CHPE_DEV void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+CHPE_DEV void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 bytes global -> shared; zeros when !on (the address is not read)
+CHPE_DEV void cp16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+CHPE_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+CHPE_DEV void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+CHPE_DEV float load_any(const void* p, int type, int64_t i) {
+  if (type == CHPE_F32) return static_cast<const float*>(p)[i];
+  if (type == CHPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+CHPE_DEV void store_any(void* p, int type, int64_t i, float v) {
+  if (type == CHPE_F32) static_cast<float*>(p)[i] = v;
+  else if (type == CHPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+CHPE_DEV int seq_len(const PagedLaunch& P, int b) {
+  const int n = P.lens[b];
+  return n <= 0 ? 0 : (int)min((int64_t)n, P.cap);
+}
+CHPE_DEV int tiles_of(int len) { return len / kTile + (len % kTile != 0); }
+
+template <int D>
+struct Cfg {
+  static constexpr int kRow = D * 2;                  // bytes of a cache row of one head
+  static constexpr int kStageBytes = 2 * kUnit * kRow;  // K and V of one unit
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kRec = D + 2;                  // floats of a record of one head: values, max, sum
+};
+
+// NP: passes over the query's parts (1: hi + lo; 2: a third part for float
+// queries over a BF16 cache, with the probability in three parts too).
+template <typename T, int D, int NP>
+__global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
+  using C = Cfg<D>;
+  constexpr int KS = D / 16, NT = D / 8, CH = D / 8;  // k steps, output n-tiles, 16-byte chunks per row
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ long long strip_sum[kWarps];
+  __shared__ long long s_base;
+  __shared__ int s_seq;
+  __shared__ float wm[kWarps][kHeads], wl[kWarps][kHeads];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row = lane >> 2, quad = lane & 3;
+  const int cta = blockIdx.x, n_cta = gridDim.x;
+
+  // ---- this CTA's stretch of the line of tiles
+  const int per = (P.B + 32 * kWarps - 1) / (32 * kWarps);
+  const int b_lo = min(tid * per, P.B), b_hi = min(b_lo + per, P.B);
+  long long mine = 0;
+  for (int b = b_lo; b < b_hi; b++) mine += tiles_of(seq_len(P, b));
+  mine *= P.VH;
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) strip_sum[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) {
+    before += w < warp ? strip_sum[w] : 0;
+    total += strip_sum[w];
+  }
+  incl += before;
+  const long long share = total / n_cta, more = total % n_cta;
+  const long long t_begin = cta * share + min((long long)cta, more);
+  const long long t_end = t_begin + share + (cta < more ? 1 : 0);
+  if (t_begin < t_end && t_begin >= incl - mine && t_begin < incl) {  // one thread
+    long long base = incl - mine;
+    int b = b_lo;
+    for (; b < b_hi - 1; b++) {
+      const long long n = (long long)tiles_of(seq_len(P, b)) * P.VH;
+      if (t_begin < base + n) break;
+      base += n;
+    }
+    s_seq = b;
+    s_base = base;
+  }
+  // sequences without a position: nothing else writes their outputs
+  for (int b = cta; b < P.B; b += n_cta) {
+    if (seq_len(P, b) > 0) continue;
+    for (int i = tid; i < P.H * D; i += 32 * kWarps) store_any(P.out, P.q_type, b * P.out_stride + i, 0.f);
+    if (P.lse)
+      for (int i = tid; i < P.H; i += 32 * kWarps) P.lse[(int64_t)b * P.H + i] = -INFINITY;
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  if (t_begin >= t_end) {
+    if (tid == 0) P.desc[cta] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  int b = s_seq;
+  long long base = s_base;
+  int len = seq_len(P, b), tiles = tiles_of(len);
+  int4 cut = make_int4(0, 0, 0, 0);
+
+  const uint32_t ring = smem_u32(smem) + warp * (C::kStages * C::kStageBytes);
+  const size_t row_stride = (size_t)P.KV * D;  // elements between positions
+  const T* const kc = static_cast<const T*>(P.kc);
+  const T* const vc = static_cast<const T*>(P.vc);
+
+  for (long long t = t_begin; t < t_end;) {
+    while (t >= base + (long long)tiles * P.VH) {  // the next sequence that has tiles
+      base += (long long)tiles * P.VH;
+      len = seq_len(P, ++b);
+      tiles = tiles_of(len);
+    }
+    const int vh = (int)((t - base) / tiles), tile0 = (int)((t - base) % tiles);
+    const int n_tiles = (int)min((long long)(tiles - tile0), t_end - t);
+    const int kvh = vh / P.HT, h0 = kvh * P.G + (vh % P.HT) * kHeads;
+    const int nh = min(kHeads, (kvh + 1) * P.G - h0);
+
+    // ---- issue of one unit: rows [p, p+16) of this warp
+    const int32_t* const trow = P.table + b * P.table_stride;
+    int page_at = -1, page_val = 0;
+    auto page_of = [&](int it) {  // page of unit `it`; lanes hold 32 units' pages at a time
+      if ((it & ~31) != page_at) {
+        page_at = it & ~31;
+        const int64_t p = (int64_t)(tile0 + page_at + lane) * kTile + warp * kUnit;
+        page_val = p < len ? trow[p >> P.page_shift] : -1;
+      }
+      const int pg = __shfl_sync(0xffffffffu, page_val, it & 31);
+      return (uint32_t)pg < P.n_pages ? pg : -1;
+    };
+    uint32_t ok_bits = 0;  // by stage: the unit's page is valid
+    auto issue = [&](int it) {
+      if (it < n_tiles) {
+        const int p = (tile0 + it) * kTile + warp * kUnit;
+        const int pg = page_of(it);
+        const int st = it % C::kStages;
+        ok_bits = (ok_bits & ~(1u << st)) | ((pg >= 0 ? 1u : 0u) << st);
+        const size_t r0 = ((size_t)(pg < 0 ? 0 : pg) << P.page_shift) + (p & ((1 << P.page_shift) - 1));
+        const T* const ks = kc + r0 * row_stride + (size_t)kvh * D;
+        const T* const vs = vc + r0 * row_stride + (size_t)kvh * D;
+        const uint32_t dst = ring + st * C::kStageBytes;
+        constexpr int VEC = kUnit * CH;  // 16-byte chunks of K (and of V)
+#pragma unroll
+        for (int i = 0; i < VEC / 32; i++) {
+          const int v = i * 32 + lane, r = v / CH, ch = v % CH;
+          const bool on = pg >= 0 && p + r < len;
+          const uint32_t d = dst + r * C::kRow + ((ch ^ (r & 7)) << 4);
+          const size_t off = on ? r * row_stride + ch * 8 : 0;
+          cp16(d, on ? ks + off : kc, on);
+          cp16(d + kUnit * C::kRow, on ? vs + off : vc, on);
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; s++) issue(s);
+
+    // ---- the query's parts as A operands: rows 0-7 hi, 8-15 lo
+    uint32_t qa[NP][KS][4];
+    float q_scale;  // back from the scaled parts, times scale * log2(e)
+    {
+      float2 x[KS][2];
+      float top = 0.f;
+      const int64_t qo = b * P.q_stride + (int64_t)(h0 + row) * D;
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int d = k * 16 + h * 8 + 2 * quad;
+          x[k][h] = row < nh ? make_float2(load_any(P.q, P.q_type, qo + d), load_any(P.q, P.q_type, qo + d + 1))
+                             : make_float2(0.f, 0.f);
+          top = fmaxf(top, fmaxf(fabsf(x[k][h].x), fabsf(x[k][h].y)));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // a power of two that brings the largest |q| of the head to [1, 2): FP16
+      // parts neither overflow nor lose small heads
+      int e = 0;
+      if (top > 0.f && top < INFINITY) e = ilogbf(top);
+      e = max(-126, min(126, e));
+      const float down = ldexpf(1.f, -e);
+      q_scale = P.scale * 1.44269504088896340736f * ldexpf(1.f, e);
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float2 y = make_float2(x[k][h].x * down, x[k][h].y * down);
+#pragma unroll
+          for (int np = 0; np < NP; np++)
+#pragma unroll
+            for (int part = 0; part < 2; part++) {
+              const uint32_t w = pack2<T>(y.x, y.y);
+              qa[np][k][2 * h + part] = w;
+              const float2 f = unpack2<T>(w);
+              y.x -= f.x;
+              y.y -= f.y;
+            }
+        }
+    }
+
+    float o[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[n][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    // ldmatrix row addresses: K (no transposition): matrices (pos 0-7, k lo), (pos
+    // 0-7, k hi), (pos 8-15, k lo), (pos 8-15, k hi); V (transposed): (pos 0-7,
+    // dims lo), (pos 8-15, dims lo), (pos 0-7, dims hi), (pos 8-15, dims hi)
+    const int mat = lane >> 3, mr = lane & 7;
+    const int k_row = (mat >> 1) * 8 + mr, k_ch = mat & 1;
+    const int v_row = (mat & 1) * 8 + mr, v_ch = mat >> 1;
+
+    for (int it = 0; it < n_tiles; it++) {
+      issue(it + C::kStages - 1);
+      cp_wait<C::kStages - 1>();
+      __syncwarp();
+      const int st = it % C::kStages;
+      const int p = (tile0 + it) * kTile + warp * kUnit;
+      if (p < len && (ok_bits >> st & 1u)) {
+        const uint32_t kb = ring + st * C::kStageBytes, vb = kb + kUnit * C::kRow;
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          uint32_t kf[4];
+          ldsm4(kf, kb + k_row * C::kRow + (((2 * k + k_ch) ^ (k_row & 7)) << 4));
+#pragma unroll
+          for (int np = 0; np < NP; np++) {
+            mma16816<T>(s[0], qa[np][k], kf[0], kf[1]);
+            mma16816<T>(s[1], qa[np][k], kf[2], kf[3]);
+          }
+        }
+        // scores of head `row`, positions p + 8 j + 2 quad + {0, 1}
+        float sc[2][2], mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const bool in = p + 8 * j + 2 * quad + e < len;
+            sc[j][e] = in ? (s[j][e] + s[j][e + 2]) * q_scale : -INFINITY;
+            mx = fmaxf(mx, sc[j][e]);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m, mx);
+        if (__any_sync(0xffffffffu, mn != m)) {
+          const float corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
+          l *= corr;
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[n][e] *= corr;
+          m = mn;
+        }
+        const float ref = (m == -INFINITY ? 0.f : m) - kPShift;
+        uint32_t pa[NP][4];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          float2 y = make_float2(exp2f(sc[j][0] - ref), exp2f(sc[j][1] - ref));
+          l += y.x + y.y;
+#pragma unroll
+          for (int np = 0; np < NP; np++)
+#pragma unroll
+            for (int part = 0; part < 2; part++) {
+              const uint32_t w = pack2<T>(y.x, y.y);
+              pa[np][2 * j + part] = w;
+              const float2 f = unpack2<T>(w);
+              y.x -= f.x;
+              y.y -= f.y;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t vf[4];
+          ldsm4t(vf, vb + v_row * C::kRow + (((n + v_ch) ^ (v_row & 7)) << 4));
+#pragma unroll
+          for (int np = 0; np < NP; np++) {
+            mma16816<T>(o[n], pa[np], vf[0], vf[1]);
+            mma16816<T>(o[n + 1], pa[np], vf[2], vf[3]);
+          }
+        }
+      }
+      __syncwarp();  // the stage may be filled again
+    }
+    cp_wait<0>();
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (quad == 0) {
+      wm[warp][row] = m;
+      wl[warp][row] = l;
+    }
+    __syncthreads();  // the rings are drained: their memory holds the warps' sums now
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) M = fmaxf(M, wm[w][row]);
+    const float back = m == -INFINITY ? 0.f : exp2f(m - M);
+    float* const acc = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      // hi and lo rows add up to the head's value
+      *reinterpret_cast<float2*>(acc + ((size_t)warp * kHeads + row) * D + n * 8 + 2 * quad) =
+          make_float2((o[n][0] + o[n][2]) * back, (o[n][1] + o[n][3]) * back);
+    }
+    __syncthreads();
+    const bool whole = tile0 == 0 && n_tiles == tiles;
+    float* const rec = P.part + (size_t)(2 * cta + (tile0 == 0 ? 1 : 0)) * kHeads * C::kRec;
+    for (int i = tid; i < nh * D; i += 32 * kWarps) {
+      const int h = i / D, d = i % D;
+      float v = 0.f, L = 0.f, top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) top = fmaxf(top, wm[w][h]);
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) {
+        v += acc[((size_t)w * kHeads + h) * D + d];
+        L += wl[w][h] * (wm[w][h] == -INFINITY ? 0.f : exp2f(wm[w][h] - top));  // a NaN sum stays
+      }
+      if (whole) {
+        store_any(P.out, P.q_type, b * P.out_stride + (int64_t)(h0 + h) * D + d, L == 0.f ? 0.f : v / L);
+        if (P.lse && d == 0)
+          P.lse[(int64_t)b * P.H + h0 + h] =
+              L == 0.f ? -INFINITY : 0.693147180559945309417f * (top + (log2f(L) - kPShift));
+      } else {
+        rec[h * C::kRec + d] = v;
+        if (d == 0) {
+          rec[h * C::kRec + D] = top;
+          rec[h * C::kRec + D + 1] = L;
+        }
+      }
+    }
+    __syncthreads();  // the next stretch fills the rings again
+    if (tile0 == 0 && n_tiles < tiles) {
+      // CTAs that hold the rest of this head's tiles follow without a gap
+      const long long last = base + (long long)(vh + 1) * tiles - 1;
+      const long long big = (share + 1) * more;  // tiles of the CTAs with one more
+      const long long owner = last < big ? last / (share + 1) : more + (last - big) / share;
+      cut = make_int4(b, vh, (int)(owner - cta) + 1, 0);
+    }
+    t += n_tiles;
+  }
+  if (tid == 0) P.desc[cta] = cut;
+}
+
+// Joins the records of the head that begins in CTA blockIdx.x and ends in a
+// later one; blockIdx.y is the query head within the tile.
+template <int D>
+__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ PagedLaunch P) {
+  using C = Cfg<D>;
+  constexpr int PER = D / 32;
+  __shared__ float sv[4][D], sl[4], sm[4];
+  pdl_wait();
+  const int4 cut = P.desc[blockIdx.x];
+  const int n = cut.z;
+  if (n == 0) return;
+  const int kvh = cut.y / P.HT, h = blockIdx.y, h0 = kvh * P.G + (cut.y % P.HT) * kHeads;
+  if (h0 + h >= (kvh + 1) * P.G) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // record i: the beginning lies in slot 1 of this CTA, the others in slot 0 of theirs
+  auto rec = [&](int i) {
+    return P.part + ((size_t)(2 * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0)) * kHeads + h) * C::kRec;
+  };
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, rec(i)[D]);
+  M = warp_max(M);
+  float v[PER] = {}, L = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < n; i += 4) {
+    const float* r = rec(i);
+    const float mi = r[D], w = mi == -INFINITY ? 0.f : exp2f(mi - M);
+    L = fmaf(r[D + 1], w, L);
+#pragma unroll
+    for (int e = 0; e < PER; e++) v[e] = fmaf(r[32 * e + lane], w, v[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < PER; e++) sv[warp][32 * e + lane] = v[e];
+  if (lane == 0) sl[warp] = L;
+  __syncthreads();
+  L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  for (int d = threadIdx.x; d < D; d += 128) {
+    const float x = (sv[0][d] + sv[1][d]) + (sv[2][d] + sv[3][d]);
+    store_any(P.out, P.q_type, cut.x * P.out_stride + (int64_t)(h0 + h) * D + d, L == 0.f ? 0.f : x / L);
+  }
+  if (P.lse && threadIdx.x == 0)
+    P.lse[(int64_t)cut.x * P.H + h0 + h] =
+        L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
+}
+
+size_t part_floats(uint32_t d) { return (size_t)2 * kMaxCtas * kHeads * (d + 2); }
+
+template <typename T, int D, int NP>
+cudaError_t launch(const PagedLaunch& P, int device, cudaStream_t s) {
+  using C = Cfg<D>;
+  // per device: SMs and resident CTAs of this kernel (one query, then kept)
+  static int grid_of[64] = {};
+  const int dev = device >= 0 && device < 64 ? device : -1;
+  int grid = dev >= 0 ? __atomic_load_n(&grid_of[dev], __ATOMIC_RELAXED) : 0;
+  if (grid == 0) {
+    int sms = 0, res = 0;
+    cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, D, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess)
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, D, NP>, 32 * kWarps, C::kRing);
+    if (e != cudaSuccess) return e;
+    grid = sms * (res < 1 ? 1 : res);
+    if (grid > kMaxCtas) grid = kMaxCtas;
+    if (dev >= 0) __atomic_store_n(&grid_of[dev], grid, __ATOMIC_RELAXED);
+  }
+  paged_kernel<T, D, NP><<<grid, 32 * kWarps, C::kRing, s>>>(P);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, P.G < kHeads ? P.G : kHeads);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel<D>, P);
+}
+
+template <typename T, int NP>
+cudaError_t launch_d(const PagedLaunch& P, uint32_t d, int device, cudaStream_t s) {
+  if (d == 64) return launch<T, 64, NP>(P, device, s);
+  if (d == 128) return launch<T, 128, NP>(P, device, s);
+  return launch<T, 256, NP>(P, device, s);
+}
+
+}  // namespace
+
+extern "C" size_t chpe_attention_decode_paged_workspace(uint32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
+  return kMaxCtas * sizeof(int4) + part_floats(head_dim) * sizeof(float);
+}
+
+extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_stride, const void* k_cache,
+                                           const void* v_cache, int cache_dtype, uint32_t num_pages,
+                                           uint32_t page_size, const int32_t* page_table, int64_t table_stride,
+                                           uint32_t max_pages, const int32_t* seq_lens, uint32_t batch, uint32_t num_heads,
+                                           uint32_t num_kv_heads, uint32_t head_dim, float scale, void* out,
+                                           int64_t out_stride, float* lse, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  chpe::ServeCall c("chpe_attention_decode_paged");
+  const size_t es = chpe::dtype_size(dtype);
+  if (!es) return c.fail(-1, "unknown dtype %lld", dtype), c.done();
+  if (cache_dtype != CHPE_F16 && cache_dtype != CHPE_BF16) return c.fail(-1, "the cache must be FP16 or BF16"), c.done();
+  if (dtype != CHPE_F32 && dtype != cache_dtype)
+    return c.fail(-1, "the cache must have the type of q unless q is float"), c.done();
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return c.fail(-1, "head_dim must be 64, 128 or 256"), c.done();
+  if (num_heads == 0 || num_kv_heads == 0 || num_heads > 65535 || num_heads % num_kv_heads != 0)
+    return c.fail(-1, "num_heads must be a multiple of num_kv_heads, at most 65535"), c.done();
+  if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)))
+    return c.fail(-1, "page_size must be a power of two from 16 to 65536"), c.done();
+  if (batch > 65535) return c.fail(-1, "batch must be at most 65535"), c.done();
+  if (batch > 1 && (table_stride < 0 || table_stride > INT64_MAX / 8 / batch ||
+                    (table_stride != 0 && table_stride < (int64_t)max_pages)))
+    return c.fail(-1, "table_stride must be 0 (one table for all) or at least max_pages"), c.done();
+  if (!(fabsf(scale) <= 1e6f)) return c.fail(-1, "scale is not a number within 1e6"), c.done();
+  const int64_t least = (int64_t)num_heads * head_dim;
+  if (batch > 1 && (q_stride < least || out_stride < least || q_stride > INT64_MAX / 8 / batch ||
+                    out_stride > INT64_MAX / 8 / batch))
+    return c.fail(-1, "q_stride and out_stride must be at least num_heads * head_dim"), c.done();
+  if (batch == 0) return c.done();
+  if (workspace_bytes < chpe_attention_decode_paged_workspace(head_dim))
+    return c.fail(-2, "needs a workspace of %lld bytes, got %lld",
+                  (long long)chpe_attention_decode_paged_workspace(head_dim), (long long)workspace_bytes),
+           c.done();
+  c.ptr(q, "q", 16);
+  c.ptr(out, "out", es);
+  c.ptr(seq_lens, "seq_lens", 4);
+  c.ptr(workspace, "workspace", 16);
+  c.ptr_or_null(lse, "lse", 4);
+  if (num_pages && max_pages) {
+    c.ptr(k_cache, "k_cache", 16);
+    c.ptr(v_cache, "v_cache", 16);
+    c.ptr(page_table, "page_table", 4);
+  }
+  if (c.rc) return c.done();
+
+  PagedLaunch P{};
+  P.q = q, P.q_type = dtype, P.q_stride = q_stride;
+  P.kc = k_cache, P.vc = v_cache;
+  P.table = page_table, P.table_stride = table_stride, P.lens = seq_lens;
+  P.n_pages = num_pages;
+  while ((1u << P.page_shift) < page_size) P.page_shift++;
+  P.cap = num_pages ? (int64_t)max_pages * page_size : 0;  // an empty pool holds no position
+  if (P.cap > INT32_MAX - kTile) P.cap = INT32_MAX - kTile;
+  P.B = (int32_t)batch, P.H = (int32_t)num_heads, P.KV = (int32_t)num_kv_heads;
+  P.G = P.H / P.KV;
+  P.HT = (P.G + kHeads - 1) / kHeads;
+  P.VH = P.KV * P.HT;
+  P.scale = scale;
+  P.out = out, P.out_stride = out_stride, P.lse = lse;
+  P.desc = static_cast<int4*>(workspace);
+  P.part = reinterpret_cast<float*>(P.desc + kMaxCtas);
+  chpe::DeviceScope scope(c.device);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (cache_dtype == CHPE_F16) e = launch_d<__half, 1>(P, head_dim, c.device, s);
+  else if (dtype == CHPE_F32) e = launch_d<__nv_bfloat16, 2>(P, head_dim, c.device, s);
+  else e = launch_d<__nv_bfloat16, 1>(P, head_dim, c.device, s);
+  if (e != cudaSuccess) {
+    snprintf(c.msg, sizeof(c.msg), "launch: %s", cudaGetErrorString(e));
+    c.rc = -3;
+  }
+  return c.done();
+}

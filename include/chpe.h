@@ -306,6 +306,116 @@ int chpe_attention_decode_noalloc(const float *q, const float *k, const float *v
                                   uint32_t num_heads, uint32_t num_kv_heads, uint32_t head_dim,
                                   float rope_theta, void *stream);
 
+/* ---- operators of a batched decode step ----------------------------------- */
+
+/* What a program that serves several sequences calls around its own
+ * projections, on its own device buffers (no counterpart in the reference):
+ * chpe_qk_norm_rope fills the cache and turns the queries,
+ * chpe_attention_decode_paged reads the cache, chpe_logits_process applies the
+ * sampling rules.  They share one manner:
+ *
+ * Types: CHPE_F32, CHPE_F16, CHPE_BF16 below.  Strides count elements; a
+ * stride is not looked at where there is one row.  All arithmetic is f32 with
+ * one rounding at the store.
+ * Cache: K and V of one layer, each [num_pages][page_size][num_kv_heads]
+ * [head_dim] of FP16 or BF16, the layout of the engine's own pools; a slot is
+ * the row page * page_size + offset.  head_dim is 64, 128 or 256.
+ * Calls are asynchronous on `stream` (a cudaStream_t of the buffers' device;
+ * NULL: its default stream), allocate nothing, read nothing back and can be
+ * captured into a graph.  The buffers lie on one device, which need not be
+ * the current one.  They keep no state between calls, and calls on different
+ * streams may overlap (attention: with a workspace each).
+ * Return value: 0; -1 for an argument they refuse (NULL, misaligned or host
+ * pointers, sizes and types outside the limits), -2 for too small a workspace,
+ * -3 for a CUDA error at the launch; nothing is launched then and
+ * chpe_last_error(NULL) says why. */
+#define CHPE_F32 0
+#define CHPE_F16 1
+#define CHPE_BF16 2
+
+/* Per-head RMSNorm of q and k, rotary embedding, and the append of k and v to
+ * the cache, for num_tokens tokens (a decode step's, or a prompt's chunk).
+ *   y = x / sqrt(mean(x^2) + eps) * (weight + weight_offset)   per head
+ * with q_weight / k_weight [head_dim] float (NULL: that one is not normed);
+ * then the pair (y[i], y[i + rope_dim/2]) is rotated by the angle
+ * positions[t] * inv_freq[i], i < rope_dim/2 (rotate-half; dimensions from
+ * rope_dim on stay), rope_dim a multiple of 16 up to head_dim, 0: none.
+ * inv_freq is a HOST array of rope_dim/2 doubles within +-16, copied by the call;
+ * angles are exact for every int32 position.
+ * q [num_tokens][num_heads][head_dim], k and v [num_tokens][num_kv_heads]
+ * [head_dim], heads contiguous, tokens q_stride / k_stride / v_stride elements
+ * apart (one buffer may hold all three).  q_out gets the queries; k_out (or
+ * NULL) the keys, in q's type; k_cache and v_cache (both or neither) row
+ * slots[t] of each token's k and v.  A slot outside 0..cache_rows-1 (a padded
+ * token's -1) stores nothing.  Two tokens of a call must not share a row.
+ * q_out may be q itself with q's stride, k_out k itself; otherwise outputs
+ * must not overlap inputs.  Without a cache, v, v_cache, slots may be NULL and
+ * k_out is needed.  The cache has the type of q, k and v, or any when those
+ * are float.  Buffers and strides are multiples of 16 bytes. */
+int chpe_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, int64_t q_stride,
+                      int64_t k_stride, int64_t v_stride, uint32_t num_tokens, uint32_t num_heads,
+                      uint32_t num_kv_heads, uint32_t head_dim, const float *q_weight,
+                      const float *k_weight, float weight_offset, float eps,
+                      const int32_t *positions, const double *inv_freq, uint32_t rope_dim,
+                      void *q_out, int64_t q_out_stride, void *k_out, int64_t k_out_stride,
+                      void *k_cache, void *v_cache, int cache_dtype, uint64_t cache_rows,
+                      const int64_t *slots, void *stream);
+
+/* Decode attention of `batch` sequences, one query token each, over the paged
+ * cache:  out[b][h] = softmax_t(scale * q[b][h] . K[t]) V[t] over the entries
+ * t < seq_lens[b] (the new token's own among them: append it first), query
+ * heads h*G .. h*G+G-1 on kv head h, G = num_heads / num_kv_heads of any size.
+ * q and out [batch][num_heads][head_dim] of dtype, rows q_stride / out_stride
+ * apart (q rows multiples of 16 bytes); out must not overlap q or the cache.
+ * page_table: rows of max_pages entries, table_stride apart (0: one row for all);
+ * entry p of a row is the page of positions p*page_size ..; page_size a power of
+ * two from 16 to 65536.  Sequences may share pages.  seq_lens [batch] int32; a
+ * length above max_pages*page_size counts as that, one of 0 or less gives out = 0 and lse = -inf, and entries of
+ * a page outside 0..num_pages-1 are left out.  Nothing beyond a sequence's
+ * length is used, whatever the pages hold there.  lse [batch][num_heads] float
+ * (or NULL): the natural logarithm of the softmax's sum.
+ * A query, key or value in use that is not finite makes the outputs it enters
+ * NaN or infinite.
+ * The cache has q's type, or any when q is float.  Results do not depend on
+ * timing: the same call gives the same bits.
+ * workspace: chpe_attention_decode_paged_workspace(head_dim) bytes (0 for an
+ * unsupported head_dim), 16-byte aligned, of any content; calls that may
+ * overlap on the GPU need one each. */
+size_t chpe_attention_decode_paged_workspace(uint32_t head_dim);
+int chpe_attention_decode_paged(const void *q, int dtype, int64_t q_stride, const void *k_cache,
+                                const void *v_cache, int cache_dtype, uint32_t num_pages,
+                                uint32_t page_size, const int32_t *page_table, int64_t table_stride,
+                                uint32_t max_pages, const int32_t *seq_lens, uint32_t batch,
+                                uint32_t num_heads, uint32_t num_kv_heads, uint32_t head_dim, float scale, void *out,
+                                int64_t out_stride, float *lse, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
+/* Penalties, biases and a grammar's mask on the logits [batch][vocab] of
+ * dtype, and the winning token.  For row b and token v, x = logits[b][v]:
+ *   1. v anywhere in the row's history:     x = x > 0 ? x / repetition : x * repetition
+ *   2. v written c > 0 times in it after the prompt: x = x - frequency * c, then x = x - presence
+ *   3. a bias entry for v:                  x = x + its value (of several the last one's)
+ *   4. the mask bit of v is 0:              x = -inf
+ * history [batch][history_stride] int32: the row's first total_lens[b] tokens (NULL:
+ * history_len; at most history_len count), the first prompt_lens[b] of them (NULL: none)
+ * the prompt.  repetition, frequency, presence [batch] float; each may be NULL
+ * and is left out then.  bias_ids / bias_values [batch][bias_stride], max_bias (<=
+ * 65535) entries per row.  Ids outside 0..vocab-1 (-1 for unused entries) are
+ * passed over in both lists.  mask [batch][mask_stride] of 32-bit words, bit v % 32
+ * of word v / 32, 1: allowed.  A bias_stride or mask_stride of 0 gives all rows the
+ * first one's.  history, the biases and the mask may each be NULL.
+ * out [batch][out_stride] float gets every x (NULL: not wanted) and may be the
+ * logits themselves where those are float with the same stride; argmax [batch]
+ * (NULL: not wanted) the lowest token of the largest x: NaN never wins, and -1
+ * means that no x is above -inf.  Each step is rounded to f32 by itself. */
+int chpe_logits_process(const void *logits, int dtype, int64_t logits_stride, uint32_t batch,
+                        uint32_t vocab, const int32_t *history, int64_t history_stride,
+                        uint32_t history_len, const int32_t *prompt_lens, const int32_t *total_lens,
+                        const float *repetition, const float *frequency, const float *presence,
+                        const int32_t *bias_ids, const float *bias_values, int64_t bias_stride,
+                        uint32_t max_bias, const uint32_t *mask, int64_t mask_stride, float *out,
+                        int64_t out_stride, int32_t *argmax, void *stream);
+
 /* ---- probes for the parity tests ------------------------------------------ */
 
 /* gemvLinear (chpe_engine.zig:1396) on the device over host vectors:
