@@ -50,7 +50,6 @@ constexpr float kPShift = 14.f;    // probabilities are held times 2^14: FP16 ke
 
 struct PagedLaunch {
   const void* q;
-  int32_t q_type;
   int64_t q_stride;
   const void *kc, *vc;
   const int32_t* table;
@@ -119,9 +118,12 @@ CHPE_DEV void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 // 16 bytes global -> shared; zeros when !on (the address is not read)
-CHPE_DEV void cp16(uint32_t dst, const void* src, bool on) {
+CHPE_DEV void cp16_if(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+CHPE_DEV void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 CHPE_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -129,15 +131,17 @@ CHPE_DEV void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-CHPE_DEV float load_any(const void* p, int type, int64_t i) {
-  if (type == CHPE_F32) return static_cast<const float*>(p)[i];
-  if (type == CHPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+// Two neighbours of a query row (their address is a multiple of their size).
+template <typename T>
+CHPE_DEV float2 load2(const T* p) {
+  if constexpr (std::is_same<T, float>::value) return *reinterpret_cast<const float2*>(p);
+  else return unpack2<T>(*reinterpret_cast<const uint32_t*>(p));
 }
-CHPE_DEV void store_any(void* p, int type, int64_t i, float v) {
-  if (type == CHPE_F32) static_cast<float*>(p)[i] = v;
-  else if (type == CHPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+template <typename T>
+CHPE_DEV void store1(T* p, float v) {
+  if constexpr (std::is_same<T, float>::value) *p = v;
+  else if constexpr (std::is_same<T, __half>::value) *p = __float2half_rn(v);
+  else *p = __float2bfloat16_rn(v);
 }
 
 CHPE_DEV int seq_len(const PagedLaunch& P, int b) {
@@ -155,17 +159,18 @@ struct Cfg {
   static constexpr int kRec = D + 2;                  // floats of a record of one head: values, max, sum
 };
 
-// NP: passes over the query's parts (1: hi + lo; 2: a third part for float
-// queries over a BF16 cache, with the probability in three parts too).
-template <typename T, int D, int NP>
+// T: type of the cache; TQ: of q and out.  Float queries over a BF16 cache take two
+// passes: four parts of the query and of the probability.
+template <typename T, typename TQ, int D>
 __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
+  constexpr int NP = std::is_same<T, __nv_bfloat16>::value && std::is_same<TQ, float>::value ? 2 : 1;
   constexpr int KS = D / 16, NT = D / 8, CH = D / 8;  // k steps, output n-tiles, 16-byte chunks per row
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long strip_sum[kWarps];
   __shared__ long long s_base;
   __shared__ int s_seq;
-  __shared__ float wm[kWarps][kHeads], wl[kWarps][kHeads];
+  __shared__ float wm[kWarps][kHeads], wl[kWarps][kHeads], s_top[kHeads], s_sum[kHeads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = lane >> 2, quad = lane & 3;
   const int cta = blockIdx.x, n_cta = gridDim.x;
@@ -208,7 +213,8 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
   // sequences without a position: nothing else writes their outputs
   for (int b = cta; b < P.B; b += n_cta) {
     if (seq_len(P, b) > 0) continue;
-    for (int i = tid; i < P.H * D; i += 32 * kWarps) store_any(P.out, P.q_type, b * P.out_stride + i, 0.f);
+    for (int i = tid; i < P.H * D; i += 32 * kWarps)
+      store1(static_cast<TQ*>(P.out) + b * P.out_stride + i, 0.f);
     if (P.lse)
       for (int i = tid; i < P.H; i += 32 * kWarps) P.lse[(int64_t)b * P.H + i] = -INFINITY;
   }
@@ -262,15 +268,30 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
         const T* const ks = kc + r0 * row_stride + (size_t)kvh * D;
         const T* const vs = vc + r0 * row_stride + (size_t)kvh * D;
         const uint32_t dst = ring + st * C::kStageBytes;
-        constexpr int VEC = kUnit * CH;  // 16-byte chunks of K (and of V)
+        // a warp's instruction copies RPI rows; lane: row `hi` of them, chunk `ch`
+        constexpr int RPI = 32 / CH;
+        const int hi = lane / CH, ch = lane % CH;
+        const uint32_t d0 = dst + hi * C::kRow;
+        const T* k_at = ks + hi * row_stride + ch * 8;
+        const T* v_at = vs + hi * row_stride + ch * 8;
+        if (pg >= 0 && p + kUnit <= len) {
 #pragma unroll
-        for (int i = 0; i < VEC / 32; i++) {
-          const int v = i * 32 + lane, r = v / CH, ch = v % CH;
-          const bool on = pg >= 0 && p + r < len;
-          const uint32_t d = dst + r * C::kRow + ((ch ^ (r & 7)) << 4);
-          const size_t off = on ? r * row_stride + ch * 8 : 0;
-          cp16(d, on ? ks + off : kc, on);
-          cp16(d + kUnit * C::kRow, on ? vs + off : vc, on);
+          for (int i = 0; i < kUnit / RPI; i++) {
+            const uint32_t d = d0 + i * RPI * C::kRow + (((ch ^ hi) ^ ((i * RPI) & 7)) << 4);
+            cp16(d, k_at);
+            cp16(d + kUnit * C::kRow, v_at);
+            k_at += RPI * row_stride;
+            v_at += RPI * row_stride;
+          }
+        } else {  // the sequence ends in this unit, or its page is not there: zeros
+#pragma unroll 1
+          for (int i = 0; i < kUnit / RPI; i++) {
+            const int r = i * RPI + hi;
+            const bool on = pg >= 0 && p + r < len;
+            const uint32_t d = dst + r * C::kRow + ((ch ^ (r & 7)) << 4);
+            cp16_if(d, on ? k_at + i * RPI * row_stride : kc, on);
+            cp16_if(d + kUnit * C::kRow, on ? v_at + i * RPI * row_stride : vc, on);
+          }
         }
       }
       cp_commit();
@@ -284,14 +305,12 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
     {
       float2 x[KS][2];
       float top = 0.f;
-      const int64_t qo = b * P.q_stride + (int64_t)(h0 + row) * D;
+      const TQ* const q_row = static_cast<const TQ*>(P.q) + b * P.q_stride + (int64_t)(h0 + row) * D + 2 * quad;
 #pragma unroll
       for (int k = 0; k < KS; k++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const int d = k * 16 + h * 8 + 2 * quad;
-          x[k][h] = row < nh ? make_float2(load_any(P.q, P.q_type, qo + d), load_any(P.q, P.q_type, qo + d + 1))
-                             : make_float2(0.f, 0.f);
+          x[k][h] = row < nh ? load2(q_row + k * 16 + h * 8) : make_float2(0.f, 0.f);
           top = fmaxf(top, fmaxf(fabsf(x[k][h].x), fabsf(x[k][h].y)));
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -417,6 +436,14 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; w++) M = fmaxf(M, wm[w][row]);
+    if (tid < 4 * kHeads && quad == 0) {
+      float L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; w++)
+        L += wl[w][row] * (wm[w][row] == -INFINITY ? 0.f : exp2f(wm[w][row] - M));  // a NaN sum stays
+      s_top[row] = M;
+      s_sum[row] = L;
+    }
     const float back = m == -INFINITY ? 0.f : exp2f(m - M);
     float* const acc = reinterpret_cast<float*>(smem);
 #pragma unroll
@@ -428,25 +455,22 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
     __syncthreads();
     const bool whole = tile0 == 0 && n_tiles == tiles;
     float* const rec = P.part + (size_t)(2 * cta + (tile0 == 0 ? 1 : 0)) * kHeads * C::kRec;
+    TQ* const out = static_cast<TQ*>(P.out) + b * P.out_stride + (int64_t)h0 * D;
     for (int i = tid; i < nh * D; i += 32 * kWarps) {
       const int h = i / D, d = i % D;
-      float v = 0.f, L = 0.f, top = -INFINITY;
+      float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; w++) top = fmaxf(top, wm[w][h]);
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) {
-        v += acc[((size_t)w * kHeads + h) * D + d];
-        L += wl[w][h] * (wm[w][h] == -INFINITY ? 0.f : exp2f(wm[w][h] - top));  // a NaN sum stays
-      }
+      for (int w = 0; w < kWarps; w++) v += acc[(w * kHeads + h) * D + d];
+      const float L = s_sum[h];
       if (whole) {
-        store_any(P.out, P.q_type, b * P.out_stride + (int64_t)(h0 + h) * D + d, L == 0.f ? 0.f : v / L);
+        store1(out + i, L == 0.f ? 0.f : v / L);
         if (P.lse && d == 0)
           P.lse[(int64_t)b * P.H + h0 + h] =
-              L == 0.f ? -INFINITY : 0.693147180559945309417f * (top + (log2f(L) - kPShift));
+              L == 0.f ? -INFINITY : 0.693147180559945309417f * (s_top[h] + (log2f(L) - kPShift));
       } else {
         rec[h * C::kRec + d] = v;
         if (d == 0) {
-          rec[h * C::kRec + D] = top;
+          rec[h * C::kRec + D] = s_top[h];
           rec[h * C::kRec + D + 1] = L;
         }
       }
@@ -466,7 +490,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
 
 // Joins the records of the head that begins in CTA blockIdx.x and ends in a
 // later one; blockIdx.y is the query head within the tile.
-template <int D>
+template <typename TQ, int D>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
   constexpr int PER = D / 32;
@@ -501,7 +525,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Pa
   L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
   for (int d = threadIdx.x; d < D; d += 128) {
     const float x = (sv[0][d] + sv[1][d]) + (sv[2][d] + sv[3][d]);
-    store_any(P.out, P.q_type, cut.x * P.out_stride + (int64_t)(h0 + h) * D + d, L == 0.f ? 0.f : x / L);
+    store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)(h0 + h) * D + d, L == 0.f ? 0.f : x / L);
   }
   if (P.lse && threadIdx.x == 0)
     P.lse[(int64_t)cut.x * P.H + h0 + h] =
@@ -510,7 +534,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Pa
 
 size_t part_floats(uint32_t d) { return (size_t)2 * kMaxCtas * kHeads * (d + 2); }
 
-template <typename T, int D, int NP>
+template <typename T, typename TQ, int D>
 cudaError_t launch(const PagedLaunch& P, int device, cudaStream_t s) {
   using C = Cfg<D>;
   // per device: SMs and resident CTAs of this kernel (one query, then kept)
@@ -519,16 +543,16 @@ cudaError_t launch(const PagedLaunch& P, int device, cudaStream_t s) {
   int grid = dev >= 0 ? __atomic_load_n(&grid_of[dev], __ATOMIC_RELAXED) : 0;
   if (grid == 0) {
     int sms = 0, res = 0;
-    cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, D, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
+    cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, TQ, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess)
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, D, NP>, 32 * kWarps, C::kRing);
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, TQ, D>, 32 * kWarps, C::kRing);
     if (e != cudaSuccess) return e;
     grid = sms * (res < 1 ? 1 : res);
     if (grid > kMaxCtas) grid = kMaxCtas;
     if (dev >= 0) __atomic_store_n(&grid_of[dev], grid, __ATOMIC_RELAXED);
   }
-  paged_kernel<T, D, NP><<<grid, 32 * kWarps, C::kRing, s>>>(P);
+  paged_kernel<T, TQ, D><<<grid, 32 * kWarps, C::kRing, s>>>(P);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
@@ -540,14 +564,14 @@ cudaError_t launch(const PagedLaunch& P, int device, cudaStream_t s) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<D>, P);
+  return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D>, P);
 }
 
-template <typename T, int NP>
+template <typename T, typename TQ>
 cudaError_t launch_d(const PagedLaunch& P, uint32_t d, int device, cudaStream_t s) {
-  if (d == 64) return launch<T, 64, NP>(P, device, s);
-  if (d == 128) return launch<T, 128, NP>(P, device, s);
-  return launch<T, 256, NP>(P, device, s);
+  if (d == 64) return launch<T, TQ, 64>(P, device, s);
+  if (d == 128) return launch<T, TQ, 128>(P, device, s);
+  return launch<T, TQ, 256>(P, device, s);
 }
 
 }  // namespace
@@ -584,6 +608,7 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   if (batch > 1 && (q_stride < least || out_stride < least || q_stride > INT64_MAX / 8 / batch ||
                     out_stride > INT64_MAX / 8 / batch))
     return c.fail(-1, "q_stride and out_stride must be at least num_heads * head_dim"), c.done();
+  if (batch > 1 && q_stride * es % 16 != 0) return c.fail(-1, "q_stride must be a multiple of 16 bytes"), c.done();
   if (batch == 0) return c.done();
   if (workspace_bytes < chpe_attention_decode_paged_workspace(head_dim))
     return c.fail(-2, "needs a workspace of %lld bytes, got %lld",
@@ -602,7 +627,7 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   if (c.rc) return c.done();
 
   PagedLaunch P{};
-  P.q = q, P.q_type = dtype, P.q_stride = q_stride;
+  P.q = q, P.q_stride = q_stride;
   P.kc = k_cache, P.vc = v_cache;
   P.table = page_table, P.table_stride = table_stride, P.lens = seq_lens;
   P.n_pages = num_pages;
@@ -620,9 +645,10 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   chpe::DeviceScope scope(c.device);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (cache_dtype == CHPE_F16) e = launch_d<__half, 1>(P, head_dim, c.device, s);
-  else if (dtype == CHPE_F32) e = launch_d<__nv_bfloat16, 2>(P, head_dim, c.device, s);
-  else e = launch_d<__nv_bfloat16, 1>(P, head_dim, c.device, s);
+  if (cache_dtype == CHPE_F16) e = dtype == CHPE_F32 ? launch_d<__half, float>(P, head_dim, c.device, s)
+                                                     : launch_d<__half, __half>(P, head_dim, c.device, s);
+  else e = dtype == CHPE_F32 ? launch_d<__nv_bfloat16, float>(P, head_dim, c.device, s)
+                             : launch_d<__nv_bfloat16, __nv_bfloat16>(P, head_dim, c.device, s);
   if (e != cudaSuccess) {
     snprintf(c.msg, sizeof(c.msg), "launch: %s", cudaGetErrorString(e));
     c.rc = -3;

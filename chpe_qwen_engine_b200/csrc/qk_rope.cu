@@ -17,25 +17,30 @@
 // position * 2^-65), reduced to an eighth of a turn in integers before the
 // one rounding to f32.
 //
-// Bound by memory: T*D*((2H+2KV)*act + 2KV*cache) bytes, each once.  One CTA
-// takes one token and up to kWarps * IT head groups: D/8 lanes hold a head
-// (16 or 32 bytes each, so every access is a full 128-bit one), 32*8/D heads
-// per warp and group.  A warp first issues the loads of all its groups; while
-// they are in flight one thread per rotated pair computes cos and sin, which
-// the CTA's heads share through shared memory.
+// Bound by memory: T*D*((2H+2KV)*act + 2KV*cache) bytes, each once.  A lane
+// holds both halves of its rotated pairs, 8 values each (two full 128-bit
+// accesses of 16-bit values), so the rotation needs no exchange between lanes;
+// D/16 lanes make a head, 512/D heads a group.  A warp takes one token and a run of
+// its groups: it computes the token's cos and sin once (two to four pairs per lane,
+// passed around through shared memory), keeps the norm weights in registers,
+// and issues the loads of U groups before it works on the first.  How long the runs
+// are goes by the number of tokens: one group per warp when there are few (a
+// single token of the 72B's heads is 20 warps), all of a token's when the tokens alone fill
+// the GPU and the angles are worth sharing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "device_common.cuh"
 #include "serve_common.h"
 
 namespace {
 
-constexpr int kWarps = 8, kMaxHalf = 128;
+constexpr int kWarps = 4, kMaxHalf = 128;
 
 struct QkLaunch {
   const void *q, *k, *v;
@@ -46,41 +51,48 @@ struct QkLaunch {
   float offset, eps;
   const int32_t* positions;
   int32_t half;  // rotated pairs (rope_dim / 2)
-  int32_t H, KV, heads;  // heads: H + 2 KV, or H + KV without a cache
+  int32_t H, KV;
+  int32_t gq, gkv, groups;  // groups of q, of k (and of v), of all
+  int32_t runs;             // warps per token
+  uint32_t warps;           // tokens * runs
   void *k_cache, *v_cache;
   const int64_t* slots;
   int64_t cache_rows;
-  int32_t groups_per_cta;
   uint64_t turn[kMaxHalf];  // 2^64 * inv_freq / (2 pi), modulo 2^64
 };
 
+// Eight values as they lie in memory, and as f32.
 template <typename T>
-CHPE_DEV void load8(const T* p, float (&x)[8]);
-template <>
-CHPE_DEV void load8<float>(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-template <>
-CHPE_DEV void load8<__half>(const __half* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  CHPE_DEV void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
-template <>
-CHPE_DEV void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  CHPE_DEV void zero() {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = make_uint4(0, 0, 0, 0);
   }
-}
+  CHPE_DEV void get(float (&x)[8]) const {
+    const uint32_t* u = &w[0].x;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = __uint_as_float(i < 4 ? (&w[0].x)[i] : (&w[sizeof(T) / 2 - 1].x)[i - 4]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+      }
+    }
+  }
+};
 template <typename T>
 CHPE_DEV void store8(T* p, const float (&x)[8]);
 template <>
@@ -122,97 +134,134 @@ CHPE_DEV float2 cos_sin_turn(uint64_t f) {
   return make_float2((quad == 1u || quad == 2u) ? -cc : cc, quad >= 2u ? -ss : ss);
 }
 
-// TA: type of q, k, v and the outputs; TC: type of the cache; D: head dim;
-// IT: head groups a warp holds at once.
-template <typename TA, typename TC, int D, int IT>
+// TA: type of q, k, v and the outputs; TC: type of the cache; D: head dim; U:
+// groups a warp has in flight.
+template <typename TA, typename TC, int D, int U>
 __global__ void __launch_bounds__(32 * kWarps) qk_rope_kernel(const __grid_constant__ QkLaunch P) {
-  constexpr int LPH = D / 8, HPW = 32 / LPH;  // lanes per head, heads per warp and group
-  __shared__ float2 cs[kMaxHalf];
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int LPH = D / 16, HPG = 32 / LPH;  // lanes per head, heads per group
+  __shared__ float2 cs[kWarps][kMaxHalf];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t id = blockIdx.x * kWarps + warp;
+  if (id >= P.warps) return;
+  const int64_t t = id / (uint32_t)P.runs;
+  const int run = (int)(id % (uint32_t)P.runs);
+  const int g_begin = (int)((int64_t)run * P.groups / P.runs), g_end = (int)((int64_t)(run + 1) * P.groups / P.runs);
   const int sub = lane % LPH, hl = lane / LPH;
-  const int heads = P.heads;
-  const int g0 = blockIdx.y * P.groups_per_cta;
-  const int g1 = min(g0 + P.groups_per_cta, (heads + HPW - 1) / HPW);
+  const int sh = P.half / 8;  // lanes that hold rotated pairs
+  // this lane's two chunks of 8: a rotated pair's halves, or two neighbours of the rest
+  const int ca = 8 * (sub < sh ? sub : 2 * sub), cb = 8 * (sub < sh ? sub + sh : 2 * sub + 1);
 
-  float x[IT][8];
-#pragma unroll
-  for (int u = 0; u < IT; u++) {
-    const int g = g0 + warp + u * kWarps, h = g * HPW + hl;
-    if (g < g1 && h < heads) {
-      const TA* src = h < P.H ? static_cast<const TA*>(P.q) + t * P.q_stride + (int64_t)h * D
-                      : h < P.H + P.KV ? static_cast<const TA*>(P.k) + t * P.k_stride + (int64_t)(h - P.H) * D
-                                       : static_cast<const TA*>(P.v) + t * P.v_stride + (int64_t)(h - P.H - P.KV) * D;
-      load8(src + 8 * sub, x[u]);
+  Raw8<TA> ra[U], rb[U];
+  auto head_of = [&](int g) {  // head of its kind and the kind: 0 q, 1 k, 2 v
+    const int kind = g < P.gq ? 0 : g < P.gq + P.gkv ? 1 : 2;
+    return make_int2((g - (kind == 0 ? 0 : kind == 1 ? P.gq : P.gq + P.gkv)) * HPG + hl, kind);
+  };
+  auto fetch = [&](int u, int g) {
+    const int2 h = head_of(g);
+    if (g < g_end && h.x < (h.y == 0 ? P.H : P.KV)) {
+      const TA* src = h.y == 0 ? static_cast<const TA*>(P.q) + t * P.q_stride
+                      : h.y == 1 ? static_cast<const TA*>(P.k) + t * P.k_stride
+                                 : static_cast<const TA*>(P.v) + t * P.v_stride;
+      ra[u].load(src + h.x * D + ca);
+      rb[u].load(src + h.x * D + cb);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[u][e] = 0.f;
+      ra[u].zero();
+      rb[u].zero();
     }
-  }
+  };
+#pragma unroll
+  for (int u = 0; u < U; u++) fetch(u, g_begin + u);
   const int64_t slot = P.slots ? P.slots[t] : -1;
-  if ((int)threadIdx.x < P.half)
-    cs[threadIdx.x] = cos_sin_turn((uint64_t)(int64_t)P.positions[t] * P.turn[threadIdx.x]);
-  __syncthreads();
+  const bool keep = slot >= 0 && slot < P.cache_rows;
 
-  const int sh = P.half / 8;  // lanes per rotated half
   float2 r[8];
-  {
-    const int i0 = 8 * (sub < sh ? sub : sub - sh);
-    const bool rot = sub < 2 * sh;
 #pragma unroll
-    for (int e = 0; e < 8; e++) r[e] = rot ? cs[i0 + e] : make_float2(1.f, 0.f);
-    if (sub < sh)  // the lower half subtracts
+  for (int e = 0; e < 8; e++) r[e] = make_float2(1.f, 0.f);
+  if (P.half) {
+    const uint64_t pos = (uint64_t)(int64_t)P.positions[t];
+    for (int i = lane; i < P.half; i += 32) cs[warp][(i & 7) * sh + (i >> 3)] = cos_sin_turn(pos * P.turn[i]);
+    __syncwarp();
+    if (sub < sh)
 #pragma unroll
-      for (int e = 0; e < 8; e++) r[e].y = -r[e].y;
+      for (int e = 0; e < 8; e++) r[e] = cs[warp][e * sh + sub];
   }
-  const int partner = sub < sh ? sub + sh : sub < 2 * sh ? sub - sh : sub;
+
+  float wa[8], wb[8];
+  int have = -1;  // kind whose weights are held
+  for (int g0 = g_begin; g0 < g_end; g0 += U) {
 #pragma unroll
-  for (int u = 0; u < IT; u++) {
-    const int g = g0 + warp + u * kWarps, h = g * HPW + hl;
-    if (g >= g1) break;  // uniform over the warp
-    const bool is_q = h < P.H, is_k = !is_q && h < P.H + P.KV;
-    const float* w = is_q ? P.q_weight : is_k ? P.k_weight : nullptr;
-    float ss = 0.f;
+    for (int u = 0; u < U; u++) {
+      const int g = g0 + u;
+      if (g >= g_end) break;
+      const int2 h = head_of(g);
+      float a[8], b[8];
+      ra[u].get(a);
+      rb[u].get(b);
+      fetch(u, g + U);
+      if (h.y < 2) {
+        const float* w = h.y == 0 ? P.q_weight : P.k_weight;
+        if (w) {
+          if (have != h.y) {
+            have = h.y;
 #pragma unroll
-    for (int e = 0; e < 8; e++) ss = fmaf(x[u][e], x[u][e], ss);
+            for (int e = 0; e < 8; e++) {
+              wa[e] = w[ca + e] + P.offset;
+              wb[e] = w[cb + e] + P.offset;
+            }
+          }
+          float ss = 0.f;
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (w) {
-      const float inv = 1.0f / sqrtf(ss / (float)D + P.eps);
-      float wv[8];
-      load8(w + 8 * sub, wv);
+          for (int e = 0; e < 8; e++) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[u][e] = x[u][e] * inv * (wv[e] + P.offset);
-    }
-    float y[8];
+          for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = 1.0f / sqrtf(ss * (1.0f / D) + P.eps);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float p = __shfl_sync(0xffffffffu, x[u][e], partner, LPH);
-      y[e] = is_q || is_k ? fmaf(x[u][e], r[e].x, p * r[e].y) : x[u][e];
-    }
-    if (h >= heads) continue;
-    if (is_q) {
-      store8(static_cast<TA*>(P.q_out) + t * P.qo_stride + (int64_t)h * D + 8 * sub, y);
-      continue;
-    }
-    const int kvh = is_k ? h - P.H : h - P.H - P.KV;
-    if (is_k && P.k_out) store8(static_cast<TA*>(P.k_out) + t * P.ko_stride + (int64_t)kvh * D + 8 * sub, y);
-    if (slot >= 0 && slot < P.cache_rows) {
-      TC* c = static_cast<TC*>(is_k ? P.k_cache : P.v_cache);
-      store8(c + (slot * P.KV + kvh) * D + 8 * sub, y);
+          for (int e = 0; e < 8; e++) {
+            a[e] = a[e] * inv * wa[e];
+            b[e] = b[e] * inv * wb[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float x = a[e], y = b[e];
+          a[e] = fmaf(x, r[e].x, -y * r[e].y);
+          b[e] = fmaf(y, r[e].x, x * r[e].y);
+        }
+      }
+      if (h.x >= (h.y == 0 ? P.H : P.KV)) continue;
+      if (h.y == 0) {
+        TA* o = static_cast<TA*>(P.q_out) + t * P.qo_stride + h.x * D;
+        store8(o + ca, a);
+        store8(o + cb, b);
+        continue;
+      }
+      if (h.y == 1 && P.k_out) {
+        TA* o = static_cast<TA*>(P.k_out) + t * P.ko_stride + h.x * D;
+        store8(o + ca, a);
+        store8(o + cb, b);
+      }
+      if (keep) {
+        TC* o = static_cast<TC*>(h.y == 1 ? P.k_cache : P.v_cache) + (slot * P.KV + h.x) * D;
+        store8(o + ca, a);
+        store8(o + cb, b);
+      }
     }
   }
 }
 
 template <typename TA, typename TC, int D>
 cudaError_t launch(QkLaunch& P, uint32_t tokens, cudaStream_t s) {
-  constexpr int HPW = 32 / (D / 8);
-  // without a cache the v heads have nowhere to go
-  P.heads = P.H + (P.k_cache ? 2 : 1) * P.KV;
-  const int groups = (P.heads + HPW - 1) / HPW;
-  constexpr int IT = 4;
-  int ctas = (groups + kWarps * IT - 1) / (kWarps * IT);
-  P.groups_per_cta = (groups + ctas - 1) / ctas;
-  qk_rope_kernel<TA, TC, D, IT><<<dim3(tokens, ctas), 32 * kWarps, 0, s>>>(P);
+  constexpr int HPG = 512 / D, U = 2;
+  P.gq = (P.H + HPG - 1) / HPG;
+  P.gkv = (P.KV + HPG - 1) / HPG;
+  P.groups = P.gq + (P.k_cache ? 2 : 1) * P.gkv;  // without a cache the v heads have nowhere to go
+  // about 32 warps for each of 148 SMs, at most one per group and at least one per token
+  const int64_t want = (148 * 32 + (int64_t)tokens - 1) / tokens;
+  P.runs = (int32_t)(want < 1 ? 1 : want > P.groups ? P.groups : want);
+  // (more warps than 32 bits can count: whole tokens)
+  if ((uint64_t)tokens * P.runs > 0xffffff00u) P.runs = 1;
+  P.warps = tokens * (uint32_t)P.runs;
+  qk_rope_kernel<TA, TC, D, U><<<(P.warps + kWarps - 1) / kWarps, 32 * kWarps, 0, s>>>(P);
   return cudaGetLastError();
 }
 
