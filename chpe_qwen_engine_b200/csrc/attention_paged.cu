@@ -494,7 +494,7 @@ template <typename TQ, int D>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
   constexpr int PER = D / 32;
-  __shared__ float sv[4][D], sl[4], sm[4];
+  __shared__ float sv[4][D], sl[4];
   pdl_wait();
   const int4 cut = P.desc[blockIdx.x];
   const int n = cut.z;

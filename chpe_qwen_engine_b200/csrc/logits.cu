@@ -11,34 +11,47 @@
 // is above -inf.
 //
 // Bound by memory: the logits in, the f32 logits out.  A cluster of 8 CTAs takes
-// one row, a slice of the vocabulary each.  A CTA counts its slice's tokens of the
-// history in shared memory (one word per token: bit 31 seen in the prompt, the
-// rest the count after it) with integer atomics, whose order does not matter,
-// then streams its slice once, four tokens per thread and step.  The CTAs join
-// their best tokens through distributed shared memory: no workspace, no second
-// launch.  Without history and biases no table is made.
-#include <cooperative_groups.h>
+// one row; tiles of 128 tokens (a warp's four per lane) go to the CTAs in turn, so
+// that the frequent tokens, which have low ids, are spread over them.  Three steps:
+//   1. table: the CTA's tokens of the history are counted in shared memory (one
+//      entry per token: the top bit seen in the prompt, the rest the count after it;
+//      16-bit entries unless the history is longer than they count), its biases
+//      entered.  Integer atomics, whose order does not matter; the prompt's bits are read
+//      before they are set, since many threads meet at the frequent tokens;
+//   2. stream: the CTA's tokens once, four per thread and step, kAhead steps' loads in
+//      flight (the first ones issued before step 1), the mask applied; tokens with an
+//      entry are left out of the comparison;
+//   3. rules: the tokens with an entry, which step 2 put on a list, one per thread
+//      whatever their place: their logits are worked out and written over what step 2
+//      left there.  (Worked out in step 2, a few lanes at a time with the others
+//      waiting, they took three times as long.)
+// The CTAs join their best tokens through distributed shared memory: no
+// workspace, no second launch.  Without history and biases only step 2 is left.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
+#include <type_traits>
 
 #include "device_common.cuh"
 #include "serve_common.h"
 
-namespace cg = cooperative_groups;
-
 namespace {
 
-constexpr int kCluster = 8, kThreads = 512;
-constexpr uint32_t kChunk = 32768;  // tokens of a slice counted at a time (6 bytes each with biases)
+constexpr uint32_t kCluster = 8;
+constexpr int kMaxThreads = 1024;
+constexpr uint32_t kTile = 128;
+constexpr uint32_t kChunk = 28672;  // most tokens of a CTA counted at a time (up to 8 bytes each)
+constexpr int kAhead = 4;  // steps of the stream, and
+constexpr int kIds = 4;    // ids of the history, whose loads a thread has in flight
 
 struct LogitsLaunch {
   const void* logits;
   int64_t stride;
-  uint32_t vocab, slice, chunk;  // slice: tokens per CTA; chunk: per pass over them (both multiples of 32)
+  uint32_t vocab, chunk;  // chunk: tokens a CTA takes at a time (a multiple of kTile)
   const int32_t* history;
   int64_t history_stride;
   uint32_t history_len;
@@ -61,6 +74,20 @@ CHPE_DEV unsigned long long order_key(float v, uint32_t idx) {
   return ((unsigned long long)o << 32) | (unsigned long long)(0xFFFFFFFFu - idx);
 }
 
+// ---- cluster: rank, barrier in two halves, a store to another CTA's shared memory
+CHPE_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+CHPE_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+CHPE_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+CHPE_DEV void put_cluster(unsigned long long* p, uint32_t rank, unsigned long long v) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+
 template <typename T>
 CHPE_DEV float to_float(T v);
 template <>
@@ -70,197 +97,290 @@ CHPE_DEV float to_float<__half>(__half v) { return __half2float(v); }
 template <>
 CHPE_DEV float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// Four logits as they lie in memory, and as f32.
 template <typename T>
-CHPE_DEV void load4(const T* p, float (&x)[4]);
-template <>
-CHPE_DEV void load4<float>(const float* p, float (&x)[4]) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-}
-template <>
-CHPE_DEV void load4<__half>(const __half* p, float (&x)[4]) {
-  const uint2 a = *reinterpret_cast<const uint2*>(p);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a.x));
-  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&a.y));
-  x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
-}
-template <>
-CHPE_DEV void load4<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[4]) {
-  const uint2 a = *reinterpret_cast<const uint2*>(p);
-  x[0] = __uint_as_float(a.x << 16), x[1] = __uint_as_float(a.x & 0xFFFF0000u);
-  x[2] = __uint_as_float(a.y << 16), x[3] = __uint_as_float(a.y & 0xFFFF0000u);
-}
+struct Raw4 {
+  uint32_t w[sizeof(T)];
+  CHPE_DEV void load(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p);
+      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    } else {
+      const uint2 a = *reinterpret_cast<const uint2*>(p);
+      w[0] = a.x, w[1] = a.y;
+    }
+  }
+  CHPE_DEV void get(float (&x)[4]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+  }
+};
 
-// VEC: rows and the output start at multiples of four tokens' bytes.
-template <typename T, bool HIST, bool BIAS, bool VEC>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
+// HIST: bytes of a table entry for the history (0: none).  VEC: rows and the
+// output start at multiples of four tokens' bytes.
+template <typename T, int HIST, bool BIAS, bool VEC>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
     logits_kernel(const __grid_constant__ LogitsLaunch P) {
+  constexpr bool TABLE = HIST != 0 || BIAS;
+  constexpr uint32_t kSeen = HIST == 2 ? 0x8000u : 0x80000000u;
   extern __shared__ __align__(16) unsigned char smem[];
-  uint32_t* const counts = reinterpret_cast<uint32_t*>(smem);                       // [chunk]
-  uint32_t* const which = reinterpret_cast<uint32_t*>(smem + (HIST ? 4 * P.chunk : 0));  // [chunk] 16-bit entries
-  __shared__ unsigned long long best_of[kThreads / 32];
-  __shared__ unsigned long long cta_best;
-  cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t tid = threadIdx.x, rank = cluster.block_rank();
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(smem);  // [chunk] of HIST bytes
+  uint32_t* const which = counts + P.chunk / 4 * HIST;         // [chunk] of 16 bits
+  uint16_t* const list = reinterpret_cast<uint16_t*>(which + (BIAS ? P.chunk / 2 : 0));  // tokens with an entry
+  __shared__ uint32_t listed;
+  __shared__ unsigned long long best_of[kMaxThreads / 32];
+  __shared__ unsigned long long cta_best[kCluster];
+  const uint32_t tid = threadIdx.x, rank = cluster_rank(), nt = blockDim.x;
+  if (P.argmax) cluster_arrive();  // every CTA of the cluster has started: waited for at the end
   const int64_t row = blockIdx.x / kCluster;
-  const uint32_t v_begin = min(rank * P.slice, P.vocab), v_end = min(v_begin + P.slice, P.vocab);
   const T* const x_row = static_cast<const T*>(P.logits) + row * P.stride;
   float* const out = P.out ? P.out + row * P.out_stride : nullptr;
   const uint32_t* const mask = P.mask ? P.mask + row * P.mask_stride : nullptr;
-  const float* const bias_values = BIAS ? P.bias_values + row * P.bias_stride : nullptr;
-  float rep = 1.f, freq = 0.f, pres = 0.f;
-  uint32_t total = 0, prompt = 0;
-  if (HIST) {
-    if (P.repetition) rep = P.repetition[row];
-    if (P.frequency) freq = P.frequency[row];
-    if (P.presence) pres = P.presence[row];
-    const int n = P.total_lens ? P.total_lens[row] : (int)P.history_len;
-    total = n < 0 ? 0u : min((uint32_t)n, P.history_len);
-    const int p = P.prompt_lens ? P.prompt_lens[row] : 0;
-    prompt = p < 0 ? 0u : (uint32_t)p;
-  }
+  // the CTA's i-th token, and the place of token v among them (0xFFFFFFFF: another CTA's, or none)
+  auto token = [&](uint32_t i) { return ((i / kTile) * kCluster + rank) * kTile + i % kTile; };
+  auto place = [&](uint32_t v) {
+    const uint32_t tile = v / kTile;
+    return v < P.vocab && tile % kCluster == rank ? tile / kCluster * kTile + v % kTile : 0xFFFFFFFFu;
+  };
+  const uint32_t tiles = (P.vocab + kTile - 1) / kTile;
+  const uint32_t mine = rank < tiles ? ((tiles - rank - 1) / kCluster + 1) * kTile : 0;  // the last may be cut
 
   float best = -INFINITY;
   uint32_t best_v = 0;
-  auto rule = [&](float x, uint32_t v, uint32_t word, uint32_t entry) {
-    if (HIST && word) {
-      if (P.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-      const uint32_t n = word & 0x7FFFFFFFu;
-      if (n) {
-        if (P.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)n));
-        if (P.presence) x = __fsub_rn(x, pres);
-      }
-    }
-    if (BIAS && entry) x = __fadd_rn(x, bias_values[entry - 1]);
-    return x;
-  };
-  auto offer = [&](float x, uint32_t v) {
-    if (x > best) {
+  auto offer = [&](float x, uint32_t v) {  // in any order: of equals the lowest
+    if (x > best || (x == best && v < best_v && x > -INFINITY)) {
       best = x;
       best_v = v;
     }
   };
+  for (uint32_t c0 = 0; c0 < mine; c0 += P.chunk) {
+    const uint32_t n = min(P.chunk, mine - c0);
+    Raw4<T> raw[kAhead];
+    uint32_t bits[kAhead];
+    auto fetch = [&](int u, uint32_t i) {
+      const uint32_t v = token(c0 + i);
+      if (i < n && v + 4 <= P.vocab) {
+        raw[u].load(x_row + v);
+        if (mask) bits[u] = mask[v >> 5];
+      }
+    };
+    if constexpr (VEC)
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) fetch(u, 4 * (tid + u * nt));
 
-  for (uint32_t c0 = v_begin; c0 < v_end; c0 += P.chunk) {
-    const uint32_t n = min(P.chunk, v_end - c0);
-    if constexpr (HIST || BIAS) {
-      if (c0 != v_begin) __syncthreads();  // the previous chunk's table is read
-      const uint32_t words = (HIST ? P.chunk : 0) + (BIAS ? P.chunk / 2 : 0);
-      for (uint32_t i = tid; i < words / 4; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    uint32_t total = 0, prompt = 0;
+    const int32_t* const hist = HIST ? P.history + row * P.history_stride : nullptr;
+    const int32_t* const ids = BIAS ? P.bias_ids + row * P.bias_stride : nullptr;
+    if constexpr (TABLE) {
+      if (c0) __syncthreads();  // the previous chunk's table is read
+      const uint32_t words = P.chunk / 4 * HIST + (BIAS ? P.chunk / 2 : 0);
+      for (uint32_t i = tid; i < words / 4; i += nt) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
+      if constexpr (HIST != 0) {
+        const int m = P.total_lens ? P.total_lens[row] : (int)P.history_len;
+        total = m < 0 ? 0u : min((uint32_t)m, P.history_len);
+        const int p = P.prompt_lens ? P.prompt_lens[row] : 0;
+        prompt = p < 0 ? 0u : (uint32_t)p;
+      }
+      if (tid == 0) listed = 0;
       __syncthreads();
-      if (HIST) {
-        const int32_t* const h = P.history + row * P.history_stride;
-        for (uint32_t i = tid; i < total; i += kThreads) {
-          const uint32_t o = (uint32_t)h[i] - c0;  // ids outside the slice, negative ones too, are large
-          if (o < n) {
-            if (i < prompt) atomicOr(&counts[o], 0x80000000u);
-            else atomicAdd(&counts[o], 1u);
+      if constexpr (HIST != 0) {
+        for (uint32_t i0 = tid; i0 < total; i0 += kIds * nt) {
+          uint32_t id[kIds];
+#pragma unroll
+          for (int j = 0; j < kIds; j++) id[j] = i0 + j * nt < total ? (uint32_t)hist[i0 + j * nt] : 0xFFFFFFFFu;
+#pragma unroll
+          for (int j = 0; j < kIds; j++) {
+            const uint32_t o = place(id[j]) - c0;
+            if (o >= n) continue;
+            const uint32_t sh = HIST == 2 ? (o & 1u) * 16u : 0u;
+            uint32_t* const at = counts + (HIST == 2 ? o >> 1 : o);
+            if (i0 + j * nt >= prompt) atomicAdd(at, 1u << sh);
+            else if (!(*reinterpret_cast<volatile uint32_t*>(at) & kSeen << sh)) atomicOr(at, kSeen << sh);
           }
         }
       }
-      if (BIAS) {
-        const int32_t* const ids = P.bias_ids + row * P.bias_stride;
-        for (uint32_t i = tid; i < P.max_bias; i += kThreads) {
-          const uint32_t o = (uint32_t)ids[i] - c0;
-          if (o < n) {  // the largest entry number of the token stays
-            const uint32_t sh = (o & 1u) * 16u;
-            uint32_t old = which[o >> 1];
-            while (((old >> sh) & 0xFFFFu) < i + 1) {
-              const uint32_t seen = atomicCAS(&which[o >> 1], old, (old & ~(0xFFFFu << sh)) | ((i + 1) << sh));
-              if (seen == old) break;
-              old = seen;
+      if constexpr (BIAS) {
+        for (uint32_t i = tid; i < P.max_bias; i += nt) {
+          const uint32_t o = place((uint32_t)ids[i]) - c0;
+          if (o >= n) continue;
+          const uint32_t sh = (o & 1u) * 16u;
+          uint32_t old = which[o >> 1];
+          while (((old >> sh) & 0xFFFFu) < i + 1) {  // the largest entry number of the token stays
+            const uint32_t seen = atomicCAS(&which[o >> 1], old, (old & ~(0xFFFFu << sh)) | ((i + 1) << sh));
+            if (seen == old) break;
+            old = seen;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    // bit j: token i + j of the chunk has an entry
+    auto entries4 = [&](uint32_t i) {
+      uint32_t b = 0;
+      if constexpr (HIST == 2) {
+        const uint2 c = *reinterpret_cast<const uint2*>(counts + i / 2);
+        if (c.x | c.y) b = (c.x & 0xFFFFu ? 1u : 0u) | (c.x >> 16 ? 2u : 0u) | (c.y & 0xFFFFu ? 4u : 0u) | (c.y >> 16 ? 8u : 0u);
+      }
+      if constexpr (HIST == 4) {
+        const uint4 c = *reinterpret_cast<const uint4*>(counts + i);
+        if (c.x | c.y | c.z | c.w) b = (c.x ? 1u : 0u) | (c.y ? 2u : 0u) | (c.z ? 4u : 0u) | (c.w ? 8u : 0u);
+      }
+      if constexpr (BIAS) {
+        const uint2 c = *reinterpret_cast<const uint2*>(which + i / 2);
+        if (c.x | c.y) b |= (c.x & 0xFFFFu ? 1u : 0u) | (c.x >> 16 ? 2u : 0u) | (c.y & 0xFFFFu ? 4u : 0u) | (c.y >> 16 ? 8u : 0u);
+      }
+      return b;
+    };
+
+    if constexpr (VEC) {
+      for (uint32_t i0 = 4 * tid; i0 < n; i0 += 4 * kAhead * nt) {
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const uint32_t i = i0 + 4 * u * nt, v = token(c0 + i);
+          if (i >= n || v + 4 > P.vocab) break;  // later ones are larger
+          float x[4];
+          raw[u].get(x);
+          const uint32_t allowed = bits[u] >> (i & 31u);
+          fetch(u, i + 4 * kAhead * nt);
+          if (mask) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = allowed >> j & 1u ? x[j] : -INFINITY;
+          }
+          if (out) *reinterpret_cast<float4*>(out + v) = make_float4(x[0], x[1], x[2], x[3]);
+          if constexpr (TABLE) {  // tokens that step 3 comes back to
+            const uint32_t later = entries4(i);
+            if (later) {
+              uint32_t at = atomicAdd(&listed, __popc(later));
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                if (later >> j & 1u) {
+                  x[j] = -INFINITY;
+                  list[at++] = (uint16_t)(i + j);
+                }
             }
           }
+          const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));  // passes over NaN
+          if (top > best) {  // a thread's tokens come in ascending order
+            best = top;
+            best_v = v + (x[0] == top ? 0u : x[1] == top ? 1u : x[2] == top ? 2u : 3u);
+          }
         }
       }
-      __syncthreads();
     }
-    if (VEC) {
-      const uint32_t full = n & ~3u;
-#pragma unroll 2
-      for (uint32_t i = 4 * tid; i < full; i += 4 * kThreads) {
-        const uint32_t v = c0 + i;
-        float x[4];
-        load4(x_row + v, x);
-        const uint32_t bits = mask ? mask[v >> 5] >> (v & 31u) : 0xFu;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        uint2 e = make_uint2(0, 0);
-        if (HIST) w = *reinterpret_cast<const uint4*>(counts + i);
-        if (BIAS) e = *reinterpret_cast<const uint2*>(which + (i >> 1));
-        if ((HIST && (w.x | w.y | w.z | w.w)) || (BIAS && (e.x | e.y))) {
-          x[0] = rule(x[0], v, w.x, e.x & 0xFFFFu);
-          x[1] = rule(x[1], v + 1, w.y, e.x >> 16);
-          x[2] = rule(x[2], v + 2, w.z, e.y & 0xFFFFu);
-          x[3] = rule(x[3], v + 3, w.w, e.y >> 16);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (!(bits >> j & 1u)) x[j] = -INFINITY;
-          offer(x[j], v + j);
-        }
-        if (out) *reinterpret_cast<float4*>(out + v) = make_float4(x[0], x[1], x[2], x[3]);
-      }
-    }
-    for (uint32_t i = (VEC ? (n & ~3u) : 0u) + tid; i < n; i += kThreads) {
-      const uint32_t v = c0 + i;
+    // one by one: all tokens, or those behind the last whole four
+    for (uint32_t i = VEC ? n - min(n, kTile) + tid : tid; i < n; i += nt) {
+      const uint32_t v = token(c0 + i);
+      if (v >= P.vocab || (VEC && v < (P.vocab & ~3u))) continue;
       float x = to_float<T>(x_row[v]);
-      x = rule(x, v, HIST ? counts[i] : 0u, BIAS ? (which[i >> 1] >> ((i & 1u) * 16u)) & 0xFFFFu : 0u);
       if (mask && !(mask[v >> 5] >> (v & 31u) & 1u)) x = -INFINITY;
-      offer(x, v);
       if (out) out[v] = x;
+      bool open = true;
+      if constexpr (TABLE) open = !(entries4(i & ~3u) >> (i & 3u) & 1u);
+      if (open) offer(x, v);
+      else list[atomicAdd(&listed, 1u)] = (uint16_t)i;
+    }
+
+    if constexpr (TABLE) {
+      float rep = 1.f, freq = 0.f, pres = 0.f;
+      if constexpr (HIST != 0) {
+        if (P.repetition) rep = P.repetition[row];
+        if (P.frequency) freq = P.frequency[row];
+        if (P.presence) pres = P.presence[row];
+      }
+      __syncthreads();  // step 3 writes over what other threads wrote
+      for (uint32_t k = tid; k < listed; k += nt) {
+        const uint32_t o = list[k], v = token(c0 + o);
+        float x = to_float<T>(x_row[v]);  // in place a forbidden token's logit is gone: it is -inf whatever it was
+        const uint32_t allowed = mask ? mask[v >> 5] >> (v & 31u) & 1u : 1u;
+        if constexpr (HIST != 0) {
+          const uint32_t word = HIST == 2 ? counts[o >> 1] >> ((o & 1u) * 16u) & 0xFFFFu : counts[o];
+          if (word && P.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+          const uint32_t c = word & (kSeen - 1u);
+          if (c && P.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)c));
+          if (c && P.presence) x = __fsub_rn(x, pres);
+        }
+        if constexpr (BIAS) {
+          const uint32_t e = which[o >> 1] >> ((o & 1u) * 16u) & 0xFFFFu;
+          if (e) x = __fadd_rn(x, P.bias_values[row * P.bias_stride + e - 1]);
+        }
+        if (!allowed) x = -INFINITY;
+        if (out) out[v] = x;
+        offer(x, v);
+      }
     }
   }
   if (!P.argmax) return;  // uniform over the grid
 
   unsigned long long key = best > -INFINITY ? order_key(best, best_v) : 0ull;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long k = __shfl_xor_sync(0xffffffffu, key, o);
-    key = k > key ? k : key;
-  }
-  if ((tid & 31u) == 0) best_of[tid >> 5] = key;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kThreads / 32; w++) key = best_of[w] > key ? best_of[w] : key;
-    cta_best = key;
-  }
-  cluster.sync();
-  if (rank == 0 && tid < 32) {
-    key = tid < kCluster ? *cluster.map_shared_rank(&cta_best, tid) : 0ull;
+  auto warp_key = [&] {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long k = __shfl_xor_sync(0xffffffffu, key, o);
       key = k > key ? k : key;
     }
-    if (tid == 0) P.argmax[row] = key ? (int32_t)(0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFull)) : -1;
-  }
-  cluster.sync();  // the other CTAs' shared memory stays until it is read
+  };
+  warp_key();
+  if ((tid & 31u) == 0) best_of[tid >> 5] = key;
+  __syncthreads();
+  if (tid >= 32) return;  // one warp closes the CTA; the others count as arrived
+  key = tid < nt / 32 ? best_of[tid] : 0ull;
+  warp_key();
+  cluster_wait();
+  if (tid == 0) put_cluster(&cta_best[rank], 0, key);
+  cluster_arrive();  // rank 0 alone stays for the others' keys
+  if (rank != 0) return;
+  cluster_wait();
+  key = tid < kCluster ? *reinterpret_cast<volatile unsigned long long*>(&cta_best[tid]) : 0ull;
+  warp_key();
+  if (tid == 0) P.argmax[row] = key ? (int32_t)(0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFull)) : -1;
 }
 
-template <typename T, bool HIST, bool BIAS, bool VEC>
+template <typename T, int HIST, bool BIAS, bool VEC>
 cudaError_t launch(const LogitsLaunch& P, uint32_t batch, int device, cudaStream_t s) {
-  const int bytes = (int)(P.chunk * ((HIST ? 4 : 0) + (BIAS ? 2 : 0)));
-  if (bytes > 48 * 1024) {
+  // counts, bias entries, and room on the list for every token that can have an entry
+  uint64_t entries = (HIST ? P.history_len : 0u) + (uint64_t)(BIAS ? P.max_bias : 0u);
+  if (entries > P.chunk) entries = P.chunk;
+  const int bytes = (int)(P.chunk * (HIST + (BIAS ? 2 : 0)) + 2 * entries);
+  if (bytes > 40 * 1024) {
     static int set[64] = {};  // per device: done once
     const int dev = device >= 0 && device < 64 ? device : -1;
     if (dev < 0 || !__atomic_load_n(&set[dev], __ATOMIC_RELAXED)) {
       const cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, HIST, BIAS, VEC>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)(kChunk * ((HIST ? 4 : 0) + (BIAS ? 2 : 0))));
+                                                 (int)(kChunk * (HIST + (BIAS ? 2 : 0) + 2)));
       if (e != cudaSuccess) return e;
       if (dev >= 0) __atomic_store_n(&set[dev], 1, __ATOMIC_RELAXED);
     }
   }
-  logits_kernel<T, HIST, BIAS, VEC><<<batch * kCluster, kThreads, bytes, s>>>(P);
+  int threads = batch * kCluster <= 148 ? 1024 : 256;
+  if (const char* e = getenv("CHPE_T")) threads = atoi(e);
+  logits_kernel<T, HIST, BIAS, VEC><<<batch * kCluster, threads, bytes, s>>>(P);
   return cudaGetLastError();
 }
 
 template <typename T, bool VEC>
 cudaError_t launch_rules(const LogitsLaunch& P, uint32_t batch, int device, cudaStream_t s) {
-  if (P.history && P.bias_ids) return launch<T, true, true, VEC>(P, batch, device, s);
-  if (P.history) return launch<T, true, false, VEC>(P, batch, device, s);
-  if (P.bias_ids) return launch<T, false, true, VEC>(P, batch, device, s);
-  return launch<T, false, false, VEC>(P, batch, device, s);
+  const bool wide = P.history_len > 0x7FFFu;  // more than 15 bits count
+  if (P.bias_ids) {
+    if (!P.history) return launch<T, 0, true, VEC>(P, batch, device, s);
+    return wide ? launch<T, 4, true, VEC>(P, batch, device, s) : launch<T, 2, true, VEC>(P, batch, device, s);
+  }
+  if (!P.history) return launch<T, 0, false, VEC>(P, batch, device, s);
+  return wide ? launch<T, 4, false, VEC>(P, batch, device, s) : launch<T, 2, false, VEC>(P, batch, device, s);
 }
 
 template <typename T>
@@ -320,9 +440,8 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
 
   LogitsLaunch P{};
   P.logits = logits, P.stride = logits_stride, P.vocab = vocab;
-  const uint32_t each = (uint32_t)(((uint64_t)vocab + kCluster - 1) / kCluster);
-  P.slice = (each + 31u) & ~31u;
-  P.chunk = P.slice < kChunk ? P.slice : kChunk;
+  const uint32_t tiles = (vocab + kTile - 1) / kTile, each = (tiles + kCluster - 1) / kCluster;
+  P.chunk = each < kChunk / kTile ? each * kTile : kChunk;
   if (history_len) P.history = history, P.history_stride = history_stride, P.history_len = history_len;
   P.prompt_lens = prompt_lens, P.total_lens = total_lens;
   P.repetition = repetition, P.frequency = frequency, P.presence = presence;
