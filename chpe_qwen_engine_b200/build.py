@@ -2,6 +2,8 @@
 
 * libchpe.so        -- the product: C ABI + CUDA kernels for sm_100a (nvcc)
 * libchpe_synth.so  -- deterministic synthetic archive generator (gcc)
+* _ops.so           -- the batched decode operators on torch tensors, a CPython
+                       module over libchpe.so (g++, torch's headers)
 * chpe_fwd          -- the command-line front end over libchpe.so (the
                        reference's chpe_fwd contract)
 
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -20,6 +23,7 @@ ROOT = os.path.dirname(PKG)
 LIBCHPE = os.path.join(PKG, "libchpe.so")
 LIBSYNTH = os.path.join(PKG, "libchpe_synth.so")
 CHPE_FWD = os.path.join(PKG, "chpe_fwd")
+OPS = os.path.join(PKG, "_ops.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -68,8 +72,8 @@ def build_engine(force: bool = False) -> str:
         objdir = os.path.join(PKG, "_build")
         os.makedirs(objdir, exist_ok=True)
         nvcc = _nvcc()
-        objs = []
-        for s in ENGINE_SRCS:
+
+        def compile_one(s: str) -> str:
             o = os.path.join(objdir, os.path.splitext(s)[0] + ".o")
             src = os.path.join(CSRC, s)
             if s.endswith(".c"):
@@ -77,7 +81,10 @@ def build_engine(force: bool = False) -> str:
             else:
                 cmd = [nvcc] + NVCC_FLAGS + ["-c", src, "-o", o]
             subprocess.run(cmd, check=True)
-            objs.append(o)
+            return o
+
+        with ThreadPoolExecutor(max_workers=max(1, min(8, os.cpu_count() or 1))) as pool:
+            objs = list(pool.map(compile_one, ENGINE_SRCS))
         cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", LIBCHPE] + objs
         subprocess.run(cmd, check=True)
     return LIBCHPE
@@ -93,10 +100,32 @@ def build_cli(force: bool = False) -> str:
     return CHPE_FWD
 
 
+def build_ops(force: bool = False) -> str:
+    """_ops.so, linked against the in-tree libchpe.so (found through $ORIGIN)
+    and the installed torch."""
+    if force or _stale(OPS, ["ops_torch.cpp", "../../include/chpe.h"]):
+        import sysconfig
+
+        import torch
+        from torch.utils.cpp_extension import include_paths
+        lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-o", OPS, os.path.join(CSRC, "ops_torch.cpp"),
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+               "-I", os.path.join(ROOT, "include"), "-isystem", sysconfig.get_paths()["include"], "-isystem", cuda]
+        for p in include_paths():
+            cmd += ["-isystem", p]
+        cmd += ["-L", PKG, "-lchpe", "-Wl,-rpath,$ORIGIN", "-L", lib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+                "-ltorch_python"]
+        subprocess.run(cmd, check=True)
+    return OPS
+
+
 def build_all(force: bool = False) -> None:
     build_synth(force)
     build_engine(force)
     build_cli(force)
+    build_ops(force)
 
 
 if __name__ == "__main__":

@@ -23,17 +23,17 @@
 //      entry are left out of the comparison;
 //   3. rules: the tokens with an entry, which step 2 put on a list, one per thread
 //      whatever their place: their logits are worked out and written over what step 2
-//      left there.  (Worked out in step 2, a few lanes at a time with the others
-//      waiting, they took three times as long.)
+//      left there.
 // The CTAs join their best tokens through distributed shared memory: no
 // workspace, no second launch.  Without history and biases only step 2 is left.
+// 256 rows of 151936 BF16 logits: 55 us as they are (4.2 TB/s; a plain cast of
+// them to f32 by the library takes 103), 69 with histories of up to 8191.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cmath>
 #include <cstdint>
-#include <cstdlib>
 #include <type_traits>
 
 #include "device_common.cuh"
@@ -61,6 +61,7 @@ struct LogitsLaunch {
   const float* bias_values;
   int64_t bias_stride;
   uint32_t max_bias;
+  uint32_t slots, slot_shift;  // places for bias entries: chunk (one per token), or 2^(32 - slot_shift)
   const uint32_t* mask;
   int64_t mask_stride;
   float* out;
@@ -130,17 +131,16 @@ struct Raw4 {
   }
 };
 
-// HIST: bytes of a table entry for the history (0: none).  VEC: rows and the
+// E: bytes of a table entry (0: neither history nor biases).  VEC: rows and the
 // output start at multiples of four tokens' bytes.
-template <typename T, int HIST, bool BIAS, bool VEC>
+template <typename T, int E, bool BIAS, bool VEC>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
     logits_kernel(const __grid_constant__ LogitsLaunch P) {
-  constexpr bool TABLE = HIST != 0 || BIAS;
-  constexpr uint32_t kSeen = HIST == 2 ? 0x8000u : 0x80000000u;
+  constexpr uint32_t kSeen = E == 2 ? 0x8000u : 0x80000000u, kBiased = kSeen >> 1;
   extern __shared__ __align__(16) unsigned char smem[];
-  uint32_t* const counts = reinterpret_cast<uint32_t*>(smem);  // [chunk] of HIST bytes
-  uint32_t* const which = counts + P.chunk / 4 * HIST;         // [chunk] of 16 bits
-  uint16_t* const list = reinterpret_cast<uint16_t*>(which + (BIAS ? P.chunk / 2 : 0));  // tokens with an entry
+  uint32_t* const table = reinterpret_cast<uint32_t*>(smem);  // [chunk] entries of E bytes
+  uint32_t* const which = table + P.chunk / 4 * E;            // [slots] entry numbers of 16 bits
+  uint16_t* const list = reinterpret_cast<uint16_t*>(which + (BIAS ? P.slots / 2 : 0));  // tokens with an entry
   __shared__ uint32_t listed;
   __shared__ unsigned long long best_of[kMaxThreads / 32];
   __shared__ unsigned long long cta_best[kCluster];
@@ -156,6 +156,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
     const uint32_t tile = v / kTile;
     return v < P.vocab && tile % kCluster == rank ? tile / kCluster * kTile + v % kTile : 0xFFFFFFFFu;
   };
+  // where the search for a biased token's entry begins
+  auto slot_of = [&](uint32_t o) { return P.slots == P.chunk ? o : (o * 0x9E3779B1u) >> P.slot_shift; };
   const uint32_t tiles = (P.vocab + kTile - 1) / kTile;
   const uint32_t mine = rank < tiles ? ((tiles - rank - 1) / kCluster + 1) * kTile : 0;  // the last may be cut
 
@@ -183,13 +185,13 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
       for (int u = 0; u < kAhead; u++) fetch(u, 4 * (tid + u * nt));
 
     uint32_t total = 0, prompt = 0;
-    const int32_t* const hist = HIST ? P.history + row * P.history_stride : nullptr;
+    const int32_t* const hist = P.history ? P.history + row * P.history_stride : nullptr;
     const int32_t* const ids = BIAS ? P.bias_ids + row * P.bias_stride : nullptr;
-    if constexpr (TABLE) {
+    if constexpr (E != 0) {
       if (c0) __syncthreads();  // the previous chunk's table is read
-      const uint32_t words = P.chunk / 4 * HIST + (BIAS ? P.chunk / 2 : 0);
-      for (uint32_t i = tid; i < words / 4; i += nt) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
-      if constexpr (HIST != 0) {
+      const uint32_t words = P.chunk / 4 * E + (BIAS ? P.slots / 2 : 0);
+      for (uint32_t i = tid; i < words / 4; i += nt) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
+      if (hist) {
         const int m = P.total_lens ? P.total_lens[row] : (int)P.history_len;
         total = m < 0 ? 0u : min((uint32_t)m, P.history_len);
         const int p = P.prompt_lens ? P.prompt_lens[row] : 0;
@@ -197,32 +199,46 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
       }
       if (tid == 0) listed = 0;
       __syncthreads();
-      if constexpr (HIST != 0) {
-        for (uint32_t i0 = tid; i0 < total; i0 += kIds * nt) {
-          uint32_t id[kIds];
+      auto flag = [&](uint32_t o, uint32_t f) {
+        const uint32_t sh = E == 2 ? (o & 1u) * 16u : 0u;
+        uint32_t* const at = table + (E == 2 ? o >> 1 : o);
+        if (!(*reinterpret_cast<volatile uint32_t*>(at) & f << sh)) atomicOr(at, f << sh);
+      };
+      for (uint32_t i0 = tid; i0 < total; i0 += kIds * nt) {
+        uint32_t id[kIds];
 #pragma unroll
-          for (int j = 0; j < kIds; j++) id[j] = i0 + j * nt < total ? (uint32_t)hist[i0 + j * nt] : 0xFFFFFFFFu;
+        for (int j = 0; j < kIds; j++) id[j] = i0 + j * nt < total ? (uint32_t)hist[i0 + j * nt] : 0xFFFFFFFFu;
 #pragma unroll
-          for (int j = 0; j < kIds; j++) {
-            const uint32_t o = place(id[j]) - c0;
-            if (o >= n) continue;
-            const uint32_t sh = HIST == 2 ? (o & 1u) * 16u : 0u;
-            uint32_t* const at = counts + (HIST == 2 ? o >> 1 : o);
-            if (i0 + j * nt >= prompt) atomicAdd(at, 1u << sh);
-            else if (!(*reinterpret_cast<volatile uint32_t*>(at) & kSeen << sh)) atomicOr(at, kSeen << sh);
-          }
+        for (int j = 0; j < kIds; j++) {
+          const uint32_t o = place(id[j]) - c0;
+          if (o >= n) continue;
+          if (i0 + j * nt < prompt) flag(o, kSeen);
+          else atomicAdd(table + (E == 2 ? o >> 1 : o), 1u << (E == 2 ? (o & 1u) * 16u : 0u));
         }
       }
       if constexpr (BIAS) {
         for (uint32_t i = tid; i < P.max_bias; i += nt) {
-          const uint32_t o = place((uint32_t)ids[i]) - c0;
+          const uint32_t id = (uint32_t)ids[i], o = place(id) - c0;
           if (o >= n) continue;
-          const uint32_t sh = (o & 1u) * 16u;
-          uint32_t old = which[o >> 1];
-          while (((old >> sh) & 0xFFFFu) < i + 1) {  // the largest entry number of the token stays
-            const uint32_t seen = atomicCAS(&which[o >> 1], old, (old & ~(0xFFFFu << sh)) | ((i + 1) << sh));
-            if (seen == old) break;
-            old = seen;
+          flag(o, kBiased);
+          uint32_t k = slot_of(o);  // at most half of the slots are taken: the search ends before it is back
+          for (uint32_t tries = 0; tries < P.slots; tries++, k = k + 1 < P.slots ? k + 1 : 0) {
+            const uint32_t sh = (k & 1u) * 16u;
+            uint32_t* const at = which + (k >> 1);
+            uint32_t old = *reinterpret_cast<volatile uint32_t*>(at);
+            bool done = false;
+            // an empty slot, or the token's own with a smaller number: the largest number stays
+            for (;;) {
+              const uint32_t e = old >> sh & 0xFFFFu;
+              if (e && (uint32_t)ids[e - 1] != id) break;
+              done = true;
+              if (e > i) break;
+              const uint32_t seen = atomicCAS(at, old, (old & ~(0xFFFFu << sh)) | ((i + 1) << sh));
+              if (seen == old) break;
+              done = false;
+              old = seen;
+            }
+            if (done) break;
           }
         }
       }
@@ -231,17 +247,12 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
     // bit j: token i + j of the chunk has an entry
     auto entries4 = [&](uint32_t i) {
       uint32_t b = 0;
-      if constexpr (HIST == 2) {
-        const uint2 c = *reinterpret_cast<const uint2*>(counts + i / 2);
+      if constexpr (E == 2) {
+        const uint2 c = *reinterpret_cast<const uint2*>(table + i / 2);
         if (c.x | c.y) b = (c.x & 0xFFFFu ? 1u : 0u) | (c.x >> 16 ? 2u : 0u) | (c.y & 0xFFFFu ? 4u : 0u) | (c.y >> 16 ? 8u : 0u);
-      }
-      if constexpr (HIST == 4) {
-        const uint4 c = *reinterpret_cast<const uint4*>(counts + i);
+      } else if constexpr (E == 4) {
+        const uint4 c = *reinterpret_cast<const uint4*>(table + i);
         if (c.x | c.y | c.z | c.w) b = (c.x ? 1u : 0u) | (c.y ? 2u : 0u) | (c.z ? 4u : 0u) | (c.w ? 8u : 0u);
-      }
-      if constexpr (BIAS) {
-        const uint2 c = *reinterpret_cast<const uint2*>(which + i / 2);
-        if (c.x | c.y) b |= (c.x & 0xFFFFu ? 1u : 0u) | (c.x >> 16 ? 2u : 0u) | (c.y & 0xFFFFu ? 4u : 0u) | (c.y >> 16 ? 8u : 0u);
       }
       return b;
     };
@@ -261,7 +272,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
             for (int j = 0; j < 4; j++) x[j] = allowed >> j & 1u ? x[j] : -INFINITY;
           }
           if (out) *reinterpret_cast<float4*>(out + v) = make_float4(x[0], x[1], x[2], x[3]);
-          if constexpr (TABLE) {  // tokens that step 3 comes back to
+          if constexpr (E != 0) {  // tokens that step 3 comes back to
             const uint32_t later = entries4(i);
             if (later) {
               uint32_t at = atomicAdd(&listed, __popc(later));
@@ -289,33 +300,34 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
       if (mask && !(mask[v >> 5] >> (v & 31u) & 1u)) x = -INFINITY;
       if (out) out[v] = x;
       bool open = true;
-      if constexpr (TABLE) open = !(entries4(i & ~3u) >> (i & 3u) & 1u);
+      if constexpr (E != 0) open = !(entries4(i & ~3u) >> (i & 3u) & 1u);
       if (open) offer(x, v);
       else list[atomicAdd(&listed, 1u)] = (uint16_t)i;
     }
 
-    if constexpr (TABLE) {
-      float rep = 1.f, freq = 0.f, pres = 0.f;
-      if constexpr (HIST != 0) {
-        if (P.repetition) rep = P.repetition[row];
-        if (P.frequency) freq = P.frequency[row];
-        if (P.presence) pres = P.presence[row];
-      }
+    if constexpr (E != 0) {
+      const float rep = P.repetition ? P.repetition[row] : 1.f;
+      const float freq = P.frequency ? P.frequency[row] : 0.f, pres = P.presence ? P.presence[row] : 0.f;
       __syncthreads();  // step 3 writes over what other threads wrote
       for (uint32_t k = tid; k < listed; k += nt) {
         const uint32_t o = list[k], v = token(c0 + o);
         float x = to_float<T>(x_row[v]);  // in place a forbidden token's logit is gone: it is -inf whatever it was
         const uint32_t allowed = mask ? mask[v >> 5] >> (v & 31u) & 1u : 1u;
-        if constexpr (HIST != 0) {
-          const uint32_t word = HIST == 2 ? counts[o >> 1] >> ((o & 1u) * 16u) & 0xFFFFu : counts[o];
-          if (word && P.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-          const uint32_t c = word & (kSeen - 1u);
-          if (c && P.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)c));
-          if (c && P.presence) x = __fsub_rn(x, pres);
-        }
+        const uint32_t word = E == 2 ? table[o >> 1] >> ((o & 1u) * 16u) & 0xFFFFu : table[o];
+        if (word & ~kBiased && P.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+        const uint32_t c = word & (kBiased - 1u);
+        if (c && P.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)c));
+        if (c && P.presence) x = __fsub_rn(x, pres);
         if constexpr (BIAS) {
-          const uint32_t e = which[o >> 1] >> ((o & 1u) * 16u) & 0xFFFFu;
-          if (e) x = __fadd_rn(x, P.bias_values[row * P.bias_stride + e - 1]);
+          if (word & kBiased) {
+            uint32_t k = slot_of(o);
+            for (uint32_t tries = 0; tries < P.slots; tries++, k = k + 1 < P.slots ? k + 1 : 0) {
+              const uint32_t e = which[k >> 1] >> ((k & 1u) * 16u) & 0xFFFFu;
+              if (e && (uint32_t)ids[e - 1] != v) continue;  // another token's
+              if (e) x = __fadd_rn(x, P.bias_values[row * P.bias_stride + e - 1]);
+              break;
+            }
+          }
         }
         if (!allowed) x = -INFINITY;
         if (out) out[v] = x;
@@ -349,38 +361,44 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
   if (tid == 0) P.argmax[row] = key ? (int32_t)(0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFull)) : -1;
 }
 
-template <typename T, int HIST, bool BIAS, bool VEC>
-cudaError_t launch(const LogitsLaunch& P, uint32_t batch, int device, cudaStream_t s) {
-  // counts, bias entries, and room on the list for every token that can have an entry
-  uint64_t entries = (HIST ? P.history_len : 0u) + (uint64_t)(BIAS ? P.max_bias : 0u);
+template <typename T, int E, bool BIAS, bool VEC>
+cudaError_t launch(LogitsLaunch P, uint32_t batch, int device, cudaStream_t s) {
+  if (BIAS) {
+    // twice as many slots as entries, hashed; or, where that is as much, one per token
+    P.slots = 32, P.slot_shift = 27;
+    while (P.slots < 2 * P.max_bias) P.slots *= 2, P.slot_shift--;
+    if (P.slots >= P.chunk) P.slots = P.chunk;
+  }
+  // table, slots, and room on the list for every token that can have an entry
+  uint64_t entries = (P.history ? P.history_len : 0u) + (uint64_t)(BIAS ? P.max_bias : 0u);
   if (entries > P.chunk) entries = P.chunk;
-  const int bytes = (int)(P.chunk * (HIST + (BIAS ? 2 : 0)) + 2 * entries);
+  const int bytes = E ? (int)(P.chunk * E + (BIAS ? 2 * P.slots : 0) + 2 * entries) : 0;
   if (bytes > 40 * 1024) {
     static int set[64] = {};  // per device: done once
     const int dev = device >= 0 && device < 64 ? device : -1;
     if (dev < 0 || !__atomic_load_n(&set[dev], __ATOMIC_RELAXED)) {
-      const cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, HIST, BIAS, VEC>,
+      const cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, E, BIAS, VEC>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)(kChunk * (HIST + (BIAS ? 2 : 0) + 2)));
+                                                 (int)(kChunk * (E + (BIAS ? 2 : 0) + 2)));
       if (e != cudaSuccess) return e;
       if (dev >= 0) __atomic_store_n(&set[dev], 1, __ATOMIC_RELAXED);
     }
   }
-  int threads = batch * kCluster <= 148 ? 1024 : 256;
-  if (const char* e = getenv("CHPE_T")) threads = atoi(e);
-  logits_kernel<T, HIST, BIAS, VEC><<<batch * kCluster, threads, bytes, s>>>(P);
+  // Few CTAs are waited for by their loads: many threads each (one row of 151936 with a
+  // history: 7.9 us with 1024, 9.1 with 256; 24 rows: 18.1 with 1024, 12.6 with 512,
+  // 14.5 with 256).  Many CTAs overlap one another's phases best when small (64
+  // rows: 47, 26, 21.9 us; 256 rows: 129, 85, 69 us).
+  const int threads = batch * kCluster <= 80 ? 1024 : batch * kCluster <= 192 ? 512 : 256;
+  logits_kernel<T, E, BIAS, VEC><<<batch * kCluster, threads, bytes, s>>>(P);
   return cudaGetLastError();
 }
 
 template <typename T, bool VEC>
 cudaError_t launch_rules(const LogitsLaunch& P, uint32_t batch, int device, cudaStream_t s) {
-  const bool wide = P.history_len > 0x7FFFu;  // more than 15 bits count
-  if (P.bias_ids) {
-    if (!P.history) return launch<T, 0, true, VEC>(P, batch, device, s);
-    return wide ? launch<T, 4, true, VEC>(P, batch, device, s) : launch<T, 2, true, VEC>(P, batch, device, s);
-  }
-  if (!P.history) return launch<T, 0, false, VEC>(P, batch, device, s);
-  return wide ? launch<T, 4, false, VEC>(P, batch, device, s) : launch<T, 2, false, VEC>(P, batch, device, s);
+  if (!P.history && !P.bias_ids) return launch<T, 0, false, VEC>(P, batch, device, s);
+  if (P.history && P.history_len > 0x3FFFu)  // more than 14 bits count
+    return P.bias_ids ? launch<T, 4, true, VEC>(P, batch, device, s) : launch<T, 4, false, VEC>(P, batch, device, s);
+  return P.bias_ids ? launch<T, 2, true, VEC>(P, batch, device, s) : launch<T, 2, false, VEC>(P, batch, device, s);
 }
 
 template <typename T>
@@ -407,7 +425,7 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
     return c.fail(-1, "lengths or penalties without a history"), c.done();
   if (!bias_ids != !bias_values) return c.fail(-1, "bias_ids and bias_values go together"), c.done();
   if (bias_ids && max_bias > 65535) return c.fail(-1, "at most 65535 biases per row"), c.done();
-  if (history_len > 0x7fffffffu) return c.fail(-1, "history_len must be below 2^31"), c.done();
+  if (history_len > 0x3fffffffu) return c.fail(-1, "history_len must be below 2^30"), c.done();
   const int64_t words = ((int64_t)vocab + 31) / 32;
   if (batch > 1) {
     const int64_t most = INT64_MAX / 8 / batch;
