@@ -8,20 +8,25 @@
 // Query heads h*G .. h*G+G-1 share kv head h.  Bound by memory: every K and V
 // row is read once, 4*H/KV flops for each 2 elements.
 //
-// Work split.  The work is a line of tiles of 64 positions: sequence by
-// sequence, head by head, tile by tile.  CTA c of C takes the c-th of C equal
-// stretches, whatever sequences lie in it, so a batch of very different
-// lengths, one long sequence and many short ones all fill the GPU alike and
-// the host never learns a length (a captured graph stays valid as sequences
-// grow).  A (sequence, head) that lies in one CTA is finished there; of one
-// cut between CTAs each writes a partial record (values, maximum, sum) and
-// combine_kernel, launched behind with programmatic dependent launch, joins the records in
-// the order of the positions: results do not depend on timing.
+// Work split.  A CTA takes several kv heads of the same positions at once, a warp
+// each, because a position's heads lie side by side in the cache: what a CTA reads
+// is then whole pages, not a 256-byte row of every 2 KB (one head per CTA, all else
+// alike: 162 us instead of @FULL for a batch of 64 on 64/8 heads of 128).  Where there are
+// fewer heads than warps the remaining warps take further 16-position units of
+// the tile.  The work is a line of tiles: sequence by sequence, group of heads by
+// group, tile by tile, and CTA c of C takes the c-th of C equal stretches,
+// whatever sequences lie in it.  A batch of very different lengths, one long
+// sequence and many short ones all fill the GPU alike, and the host never learns
+// a length (a captured graph stays valid as sequences grow).  A sequence's group that
+// lies in one CTA is finished there; of one cut between CTAs each writes partial
+// records (values, maximum, sum per query head) and combine_kernel, launched behind with
+// programmatic dependent launch, joins them in the order of the positions: results do
+// not depend on timing.
 //
-// Inside a CTA the four warps take the four 16-position units of a tile, each
-// with a ring of its own in shared memory (cp.async, 16-byte chunks XOR-swizzled
-// by row so that ldmatrix is free of bank conflicts) and a running maximum of
-// its own; they meet once per stretch.
+// Each warp has a ring of its own in shared memory (cp.async, 16-byte chunks
+// XOR-swizzled by row so that ldmatrix is free of bank conflicts), a running
+// maximum and sums in registers, and waits for no other warp; only warps that
+// share a head meet, at the end of a stretch.
 //
 // Matrix instructions: mma.sync m16n8k16.  A batch-1 product has 8 query heads
 // at most per tile against 16 rows of the instruction; the spare 8 rows carry the low
@@ -43,9 +48,8 @@
 
 namespace {
 
-constexpr int kWarps = 4, kUnit = 16, kTile = kWarps * kUnit;
-constexpr int kHeads = 8;          // query heads of one tile (a "virtual" kv head)
-constexpr int kMaxCtas = 512;      // grid limit, sizes the workspace
+constexpr int kUnit = 16;          // positions a warp takes at a time
+constexpr int kHeads = 8;          // query heads of one warp (a "virtual" kv head)
 constexpr float kPShift = 14.f;    // probabilities are held times 2^14: FP16 keeps small ones
 
 struct PagedLaunch {
@@ -57,13 +61,16 @@ struct PagedLaunch {
   const int32_t* lens;
   uint32_t n_pages, page_shift;
   int64_t cap;  // positions a table row can hold
-  int32_t B, H, KV, G, HT, VH;  // VH = KV * HT virtual heads of up to 8 query heads
+  int32_t B, H, KV, G, HT;  // HT: virtual heads (of up to 8 query heads) per kv head
+  int32_t HW, groups;       // virtual heads of a CTA (a power of two); groups of them
+  int32_t tile;             // positions of a tile: 16 for each warp that shares a head
   float scale;
   void* out;
   int64_t out_stride;
   float* lse;
-  float* part;  // [2 * grid][8][D + 2]
-  int4* desc;   // [grid]: sequence, virtual head, number of records, unused
+  float* part;  // records [2 * grid][HW][8][D + 2]
+  int4* desc;   // cuts: sequence, group, number of CTAs (0: not cut), the first of them
+  int32_t by_seq;  // a desc entry for each sequence and group (they are at most `grid`); else for each CTA
 };
 
 template <typename T>
@@ -138,6 +145,11 @@ CHPE_DEV float2 load2(const T* p) {
   else return unpack2<T>(*reinterpret_cast<const uint32_t*>(p));
 }
 template <typename T>
+CHPE_DEV void store2(T* p, float a, float b) {
+  if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float2*>(p) = make_float2(a, b);
+  else *reinterpret_cast<uint32_t*>(p) = pack2<T>(a, b);
+}
+template <typename T>
 CHPE_DEV void store1(T* p, float v) {
   if constexpr (std::is_same<T, float>::value) *p = v;
   else if constexpr (std::is_same<T, __half>::value) *p = __float2half_rn(v);
@@ -148,39 +160,42 @@ CHPE_DEV int seq_len(const PagedLaunch& P, int b) {
   const int n = P.lens[b];
   return n <= 0 ? 0 : (int)min((int64_t)n, P.cap);
 }
-CHPE_DEV int tiles_of(int len) { return len / kTile + (len % kTile != 0); }
+CHPE_DEV int tiles_of(const PagedLaunch& P, int len) { return len / P.tile + (len % P.tile != 0); }
 
 template <int D>
 struct Cfg {
-  static constexpr int kRow = D * 2;                  // bytes of a cache row of one head
+  static constexpr int kWarps = D == 256 ? 4 : 8;
+  static constexpr int kRow = D * 2;                    // bytes of a cache row of one head
   static constexpr int kStageBytes = 2 * kUnit * kRow;  // K and V of one unit
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kRec = D + 2;                  // floats of a record of one head: values, max, sum
+  static constexpr int kRec = D + 2;                    // floats of a record of one head: values, max, sum
+  static constexpr int kMaxCtas = D == 64 ? 320 : 160;  // grid limit, sizes the workspace
 };
 
 // T: type of the cache; TQ: of q and out.  Float queries over a BF16 cache take two
 // passes: four parts of the query and of the probability.
 template <typename T, typename TQ, int D>
-__global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
+__global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
   constexpr int NP = std::is_same<T, __nv_bfloat16>::value && std::is_same<TQ, float>::value ? 2 : 1;
   constexpr int KS = D / 16, NT = D / 8, CH = D / 8;  // k steps, output n-tiles, 16-byte chunks per row
+  constexpr int W = C::kWarps, THREADS = 32 * W;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long strip_sum[kWarps];
+  __shared__ long long strip_sum[W];
   __shared__ long long s_base;
   __shared__ int s_seq;
-  __shared__ float wm[kWarps][kHeads], wl[kWarps][kHeads], s_top[kHeads], s_sum[kHeads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = lane >> 2, quad = lane & 3;
   const int cta = blockIdx.x, n_cta = gridDim.x;
+  const int hw = warp & (P.HW - 1), sub = warp / P.HW, subs = W / P.HW;
 
   // ---- this CTA's stretch of the line of tiles
-  const int per = (P.B + 32 * kWarps - 1) / (32 * kWarps);
+  const int per = (P.B + THREADS - 1) / THREADS;
   const int b_lo = min(tid * per, P.B), b_hi = min(b_lo + per, P.B);
   long long mine = 0;
-  for (int b = b_lo; b < b_hi; b++) mine += tiles_of(seq_len(P, b));
-  mine *= P.VH;
+  for (int b = b_lo; b < b_hi; b++) mine += tiles_of(P, seq_len(P, b));
+  mine *= P.groups;
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -191,7 +206,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; w++) {
+  for (int w = 0; w < W; w++) {
     before += w < warp ? strip_sum[w] : 0;
     total += strip_sum[w];
   }
@@ -203,7 +218,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
     long long base = incl - mine;
     int b = b_lo;
     for (; b < b_hi - 1; b++) {
-      const long long n = (long long)tiles_of(seq_len(P, b)) * P.VH;
+      const long long n = (long long)tiles_of(P, seq_len(P, b)) * P.groups;
       if (t_begin < base + n) break;
       base += n;
     }
@@ -213,21 +228,22 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
   // sequences without a position: nothing else writes their outputs
   for (int b = cta; b < P.B; b += n_cta) {
     if (seq_len(P, b) > 0) continue;
-    for (int i = tid; i < P.H * D; i += 32 * kWarps)
-      store1(static_cast<TQ*>(P.out) + b * P.out_stride + i, 0.f);
+    for (int i = tid; i < P.H * D; i += THREADS) store1(static_cast<TQ*>(P.out) + b * P.out_stride + i, 0.f);
     if (P.lse)
-      for (int i = tid; i < P.H; i += 32 * kWarps) P.lse[(int64_t)b * P.H + i] = -INFINITY;
+      for (int i = tid; i < P.H; i += THREADS) P.lse[(int64_t)b * P.H + i] = -INFINITY;
+    if (P.by_seq)
+      for (int g = tid; g < P.groups; g += THREADS) P.desc[b * P.groups + g] = make_int4(0, 0, 0, 0);
   }
   __syncthreads();
   pdl_launch_dependents();
+  int4 cut = make_int4(0, 0, 0, 0);
   if (t_begin >= t_end) {
-    if (tid == 0) P.desc[cta] = make_int4(0, 0, 0, 0);
+    if (tid == 0 && !P.by_seq) P.desc[cta] = cut;
     return;
   }
   int b = s_seq;
   long long base = s_base;
-  int len = seq_len(P, b), tiles = tiles_of(len);
-  int4 cut = make_int4(0, 0, 0, 0);
+  int len = seq_len(P, b), tiles = tiles_of(P, len);
 
   const uint32_t ring = smem_u32(smem) + warp * (C::kStages * C::kStageBytes);
   const size_t row_stride = (size_t)P.KV * D;  // elements between positions
@@ -235,15 +251,16 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
   const T* const vc = static_cast<const T*>(P.vc);
 
   for (long long t = t_begin; t < t_end;) {
-    while (t >= base + (long long)tiles * P.VH) {  // the next sequence that has tiles
-      base += (long long)tiles * P.VH;
+    while (t >= base + (long long)tiles * P.groups) {  // the next sequence that has tiles
+      base += (long long)tiles * P.groups;
       len = seq_len(P, ++b);
-      tiles = tiles_of(len);
+      tiles = tiles_of(P, len);
     }
-    const int vh = (int)((t - base) / tiles), tile0 = (int)((t - base) % tiles);
+    const int group = (int)((t - base) / tiles), tile0 = (int)((t - base) % tiles);
     const int n_tiles = (int)min((long long)(tiles - tile0), t_end - t);
-    const int kvh = vh / P.HT, h0 = kvh * P.G + (vh % P.HT) * kHeads;
+    const int vh = group * P.HW + hw, kvh = vh / P.HT, h0 = kvh * P.G + (vh % P.HT) * kHeads;
     const int nh = min(kHeads, (kvh + 1) * P.G - h0);
+    const int p0 = tile0 * P.tile + sub * kUnit;  // this warp's first unit
 
     // ---- issue of one unit: rows [p, p+16) of this warp
     const int32_t* const trow = P.table + b * P.table_stride;
@@ -251,7 +268,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
     auto page_of = [&](int it) {  // page of unit `it`; lanes hold 32 units' pages at a time
       if ((it & ~31) != page_at) {
         page_at = it & ~31;
-        const int64_t p = (int64_t)(tile0 + page_at + lane) * kTile + warp * kUnit;
+        const int64_t p = p0 + (int64_t)(page_at + lane) * P.tile;
         page_val = p < len ? trow[p >> P.page_shift] : -1;
       }
       const int pg = __shfl_sync(0xffffffffu, page_val, it & 31);
@@ -260,7 +277,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
     uint32_t ok_bits = 0;  // by stage: the unit's page is valid
     auto issue = [&](int it) {
       if (it < n_tiles) {
-        const int p = (tile0 + it) * kTile + warp * kUnit;
+        const int p = p0 + it * P.tile;
         const int pg = page_of(it);
         const int st = it % C::kStages;
         ok_bits = (ok_bits & ~(1u << st)) | ((pg >= 0 ? 1u : 0u) << st);
@@ -359,7 +376,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
       cp_wait<C::kStages - 1>();
       __syncwarp();
       const int st = it % C::kStages;
-      const int p = (tile0 + it) * kTile + warp * kUnit;
+      const int p = p0 + it * P.tile;
       if (p < len && (ok_bits >> st & 1u)) {
         const uint32_t kb = ring + st * C::kStageBytes, vb = kb + kUnit * C::kRow;
         float s[2][4] = {};
@@ -426,118 +443,132 @@ __global__ void __launch_bounds__(32 * kWarps) paged_kernel(const __grid_constan
       __syncwarp();  // the stage may be filled again
     }
     cp_wait<0>();
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (quad == 0) {
-      wm[warp][row] = m;
-      wl[warp][row] = l;
-    }
-    __syncthreads();  // the rings are drained: their memory holds the warps' sums now
-    float M = -INFINITY;
+    if (subs > 1) {  // warps that share the head: the first one takes the others' sums
+      __syncthreads();  // every ring is drained: their memory holds the sums now
+      constexpr int kSums = NT * 64 + 64;  // floats of a warp: a pair per lane and n-tile, m and l
+      float* const mine_at = reinterpret_cast<float*>(smem) + (size_t)warp * kSums + 2 * lane;
+      if (sub > 0) {
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) M = fmaxf(M, wm[w][row]);
-    if (tid < 4 * kHeads && quad == 0) {
-      float L = 0.f;
+        for (int n = 0; n < NT; n++)
+          *reinterpret_cast<float2*>(mine_at + n * 64) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+        *reinterpret_cast<float2*>(mine_at + NT * 64) = make_float2(m, l);
+      }
+      __syncthreads();
+      if (sub == 0) {
+        for (int w = 1; w < subs; w++) {
+          const float* const at = mine_at + (size_t)w * P.HW * kSums;
+          const float2 ml = *reinterpret_cast<const float2*>(at + NT * 64);
+          const float top = fmaxf(m, ml.x);
+          const float fa = m == -INFINITY ? 0.f : exp2f(m - top), fb = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+          l = l * fa + ml.y * fb;
+          m = top;
 #pragma unroll
-      for (int w = 0; w < kWarps; w++)
-        L += wl[w][row] * (wm[w][row] == -INFINITY ? 0.f : exp2f(wm[w][row] - M));  // a NaN sum stays
-      s_top[row] = M;
-      s_sum[row] = L;
-    }
-    const float back = m == -INFINITY ? 0.f : exp2f(m - M);
-    float* const acc = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      // hi and lo rows add up to the head's value
-      *reinterpret_cast<float2*>(acc + ((size_t)warp * kHeads + row) * D + n * 8 + 2 * quad) =
-          make_float2((o[n][0] + o[n][2]) * back, (o[n][1] + o[n][3]) * back);
-    }
-    __syncthreads();
-    const bool whole = tile0 == 0 && n_tiles == tiles;
-    float* const rec = P.part + (size_t)(2 * cta + (tile0 == 0 ? 1 : 0)) * kHeads * C::kRec;
-    TQ* const out = static_cast<TQ*>(P.out) + b * P.out_stride + (int64_t)h0 * D;
-    for (int i = tid; i < nh * D; i += 32 * kWarps) {
-      const int h = i / D, d = i % D;
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) v += acc[(w * kHeads + h) * D + d];
-      const float L = s_sum[h];
-      if (whole) {
-        store1(out + i, L == 0.f ? 0.f : v / L);
-        if (P.lse && d == 0)
-          P.lse[(int64_t)b * P.H + h0 + h] =
-              L == 0.f ? -INFINITY : 0.693147180559945309417f * (s_top[h] + (log2f(L) - kPShift));
-      } else {
-        rec[h * C::kRec + d] = v;
-        if (d == 0) {
-          rec[h * C::kRec + D] = s_top[h];
-          rec[h * C::kRec + D + 1] = L;
+          for (int n = 0; n < NT; n++) {
+            const float2 v = *reinterpret_cast<const float2*>(at + n * 64);
+            o[n][0] = (o[n][0] + o[n][2]) * fa + v.x * fb;
+            o[n][1] = (o[n][1] + o[n][3]) * fa + v.y * fb;
+            o[n][2] = o[n][3] = 0.f;
+          }
         }
       }
+      __syncthreads();  // the next stretch fills the rings again
     }
-    __syncthreads();  // the next stretch fills the rings again
-    if (tile0 == 0 && n_tiles < tiles) {
-      // CTAs that hold the rest of this head's tiles follow without a gap
-      const long long last = base + (long long)(vh + 1) * tiles - 1;
-      const long long big = (share + 1) * more;  // tiles of the CTAs with one more
-      const long long owner = last < big ? last / (share + 1) : more + (last - big) / share;
-      cut = make_int4(b, vh, (int)(owner - cta) + 1, 0);
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (sub == 0 && row < nh) {
+      if (n_tiles == tiles) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        TQ* const out = static_cast<TQ*>(P.out) + b * P.out_stride + (int64_t)(h0 + row) * D + 2 * quad;
+#pragma unroll
+        for (int n = 0; n < NT; n++) store2(out + n * 8, (o[n][0] + o[n][2]) * inv, (o[n][1] + o[n][3]) * inv);
+        if (P.lse && quad == 0)
+          P.lse[(int64_t)b * P.H + h0 + row] =
+              l == 0.f ? -INFINITY : 0.693147180559945309417f * (m + (log2f(l) - kPShift));
+      } else {
+        // hi and lo rows add up to the head's value
+        float* const rec = P.part + (((size_t)2 * cta + (tile0 == 0 ? 1 : 0)) * P.HW + hw) * kHeads * C::kRec +
+                           row * C::kRec + 2 * quad;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+          *reinterpret_cast<float2*>(rec + n * 8) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+        if (quad == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(m, l);
+      }
+    }
+    if (tile0 == 0) {
+      cut = make_int4(0, 0, 0, 0);
+      if (n_tiles < tiles) {  // the CTAs that hold the rest of the group's tiles follow without a gap
+        const long long last = base + (long long)(group + 1) * tiles - 1;
+        const long long big = (share + 1) * more;  // tiles of the CTAs with one more
+        const long long owner = last < big ? last / (share + 1) : more + (last - big) / share;
+        cut = make_int4(b, group, (int)(owner - cta) + 1, cta);
+      }
+      if (tid == 0 && P.by_seq) P.desc[b * P.groups + group] = cut;
     }
     t += n_tiles;
   }
-  if (tid == 0) P.desc[cta] = cut;
+  if (tid == 0 && !P.by_seq) P.desc[cta] = cut;
 }
 
-// Joins the records of the head that begins in CTA blockIdx.x and ends in a
-// later one; blockIdx.y is the query head within the tile.
+// Joins the records of a cut group: blockIdx.x the desc entry, blockIdx.y the
+// query head within the group.
 template <typename TQ, int D>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
-  constexpr int PER = D / 32;
+  constexpr int PER = D / 64;  // pairs per lane
   __shared__ float sv[4][D], sl[4];
   pdl_wait();
   const int4 cut = P.desc[blockIdx.x];
   const int n = cut.z;
   if (n == 0) return;
-  const int kvh = cut.y / P.HT, h = blockIdx.y, h0 = kvh * P.G + (cut.y % P.HT) * kHeads;
-  if (h0 + h >= (kvh + 1) * P.G) return;
+  const int hw = blockIdx.y / kHeads, h = blockIdx.y % kHeads, vh = cut.y * P.HW + hw;
+  const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * kHeads + h;
+  if (head >= (kvh + 1) * P.G) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // record i: the beginning lies in slot 1 of this CTA, the others in slot 0 of theirs
+  // record i: the beginning lies in slot 1 of the first CTA, the others in slot 0 of theirs
   auto rec = [&](int i) {
-    return P.part + ((size_t)(2 * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0)) * kHeads + h) * C::kRec;
+    return P.part + (((size_t)2 * (cut.w + i) + (i == 0 ? 1 : 0)) * P.HW + hw) * kHeads * C::kRec + h * C::kRec;
   };
   float M = -INFINITY;
   for (int i = lane; i < n; i += 32) M = fmaxf(M, rec(i)[D]);
   M = warp_max(M);
-  float v[PER] = {}, L = 0.f;
-#pragma unroll 4
+  float2 v[PER] = {};
+  float L = 0.f;
+#pragma unroll 8
   for (int i = warp; i < n; i += 4) {
     const float* r = rec(i);
-    const float mi = r[D], w = mi == -INFINITY ? 0.f : exp2f(mi - M);
-    L = fmaf(r[D + 1], w, L);
+    const float2 ml = *reinterpret_cast<const float2*>(r + D);
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+    L = fmaf(ml.y, w, L);
 #pragma unroll
-    for (int e = 0; e < PER; e++) v[e] = fmaf(r[32 * e + lane], w, v[e]);
+    for (int e = 0; e < PER; e++) {
+      const float2 x = *reinterpret_cast<const float2*>(r + 64 * e + 2 * lane);
+      v[e].x = fmaf(x.x, w, v[e].x);
+      v[e].y = fmaf(x.y, w, v[e].y);
+    }
   }
 #pragma unroll
-  for (int e = 0; e < PER; e++) sv[warp][32 * e + lane] = v[e];
+  for (int e = 0; e < PER; e++) *reinterpret_cast<float2*>(&sv[warp][64 * e + 2 * lane]) = v[e];
   if (lane == 0) sl[warp] = L;
   __syncthreads();
   L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
   for (int d = threadIdx.x; d < D; d += 128) {
     const float x = (sv[0][d] + sv[1][d]) + (sv[2][d] + sv[3][d]);
-    store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)(h0 + h) * D + d, L == 0.f ? 0.f : x / L);
+    store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)head * D + d, L == 0.f ? 0.f : x / L);
   }
   if (P.lse && threadIdx.x == 0)
-    P.lse[(int64_t)cut.x * P.H + h0 + h] =
-        L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
+    P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
 }
 
-size_t part_floats(uint32_t d) { return (size_t)2 * kMaxCtas * kHeads * (d + 2); }
+template <int D>
+constexpr size_t workspace_bytes_of() {
+  using C = Cfg<D>;
+  return C::kMaxCtas * sizeof(int4) + (size_t)2 * C::kMaxCtas * C::kWarps * kHeads * C::kRec * sizeof(float);
+}
 
 template <typename T, typename TQ, int D>
-cudaError_t launch(const PagedLaunch& P, int device, cudaStream_t s) {
+cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   using C = Cfg<D>;
-  // per device: SMs and resident CTAs of this kernel (one query, then kept)
+  // per device: SMs times resident CTAs of this kernel (one query, then kept)
   static int grid_of[64] = {};
   const int dev = device >= 0 && device < 64 ? device : -1;
   int grid = dev >= 0 ? __atomic_load_n(&grid_of[dev], __ATOMIC_RELAXED) : 0;
@@ -546,17 +577,25 @@ cudaError_t launch(const PagedLaunch& P, int device, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, TQ, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess)
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, TQ, D>, 32 * kWarps, C::kRing);
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, TQ, D>, 32 * C::kWarps, C::kRing);
     if (e != cudaSuccess) return e;
     grid = sms * (res < 1 ? 1 : res);
-    if (grid > kMaxCtas) grid = kMaxCtas;
+    if (grid > C::kMaxCtas) grid = C::kMaxCtas;
     if (dev >= 0) __atomic_store_n(&grid_of[dev], grid, __ATOMIC_RELAXED);
   }
-  paged_kernel<T, TQ, D><<<grid, 32 * kWarps, C::kRing, s>>>(P);
+  const int vh = P.KV * P.HT;
+  P.HW = C::kWarps;
+  while (vh % P.HW != 0) P.HW /= 2;
+  P.groups = vh / P.HW;
+  P.tile = kUnit * (C::kWarps / P.HW);
+  P.by_seq = (int64_t)P.B * P.groups <= grid;
+  P.desc = static_cast<int4*>(workspace);
+  P.part = reinterpret_cast<float*>(P.desc + C::kMaxCtas);
+  paged_kernel<T, TQ, D><<<grid, 32 * C::kWarps, C::kRing, s>>>(P);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, P.G < kHeads ? P.G : kHeads);
+  cfg.gridDim = dim3(P.by_seq ? P.B * P.groups : grid, P.HW * kHeads);
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -568,17 +607,19 @@ cudaError_t launch(const PagedLaunch& P, int device, cudaStream_t s) {
 }
 
 template <typename T, typename TQ>
-cudaError_t launch_d(const PagedLaunch& P, uint32_t d, int device, cudaStream_t s) {
-  if (d == 64) return launch<T, TQ, 64>(P, device, s);
-  if (d == 128) return launch<T, TQ, 128>(P, device, s);
-  return launch<T, TQ, 256>(P, device, s);
+cudaError_t launch_d(const PagedLaunch& P, void* workspace, uint32_t d, int device, cudaStream_t s) {
+  if (d == 64) return launch<T, TQ, 64>(P, workspace, device, s);
+  if (d == 128) return launch<T, TQ, 128>(P, workspace, device, s);
+  return launch<T, TQ, 256>(P, workspace, device, s);
 }
 
 }  // namespace
 
 extern "C" size_t chpe_attention_decode_paged_workspace(uint32_t head_dim) {
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-  return kMaxCtas * sizeof(int4) + part_floats(head_dim) * sizeof(float);
+  return head_dim == 64    ? workspace_bytes_of<64>()
+         : head_dim == 128 ? workspace_bytes_of<128>()
+         : head_dim == 256 ? workspace_bytes_of<256>()
+                           : 0;
 }
 
 extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_stride, const void* k_cache,
@@ -608,14 +649,15 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   if (batch > 1 && (q_stride < least || out_stride < least || q_stride > INT64_MAX / 8 / batch ||
                     out_stride > INT64_MAX / 8 / batch))
     return c.fail(-1, "q_stride and out_stride must be at least num_heads * head_dim"), c.done();
-  if (batch > 1 && q_stride * es % 16 != 0) return c.fail(-1, "q_stride must be a multiple of 16 bytes"), c.done();
+  if (batch > 1 && (q_stride * es % 16 != 0 || out_stride * es % 16 != 0))
+    return c.fail(-1, "q_stride and out_stride must be multiples of 16 bytes"), c.done();
   if (batch == 0) return c.done();
   if (workspace_bytes < chpe_attention_decode_paged_workspace(head_dim))
     return c.fail(-2, "needs a workspace of %lld bytes, got %lld",
                   (long long)chpe_attention_decode_paged_workspace(head_dim), (long long)workspace_bytes),
            c.done();
   c.ptr(q, "q", 16);
-  c.ptr(out, "out", es);
+  c.ptr(out, "out", 16);
   c.ptr(seq_lens, "seq_lens", 4);
   c.ptr(workspace, "workspace", 16);
   c.ptr_or_null(lse, "lse", 4);
@@ -633,22 +675,19 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   P.n_pages = num_pages;
   while ((1u << P.page_shift) < page_size) P.page_shift++;
   P.cap = num_pages ? (int64_t)max_pages * page_size : 0;  // an empty pool holds no position
-  if (P.cap > INT32_MAX - kTile) P.cap = INT32_MAX - kTile;
+  if (P.cap > INT32_MAX - 1024) P.cap = INT32_MAX - 1024;
   P.B = (int32_t)batch, P.H = (int32_t)num_heads, P.KV = (int32_t)num_kv_heads;
   P.G = P.H / P.KV;
   P.HT = (P.G + kHeads - 1) / kHeads;
-  P.VH = P.KV * P.HT;
   P.scale = scale;
   P.out = out, P.out_stride = out_stride, P.lse = lse;
-  P.desc = static_cast<int4*>(workspace);
-  P.part = reinterpret_cast<float*>(P.desc + kMaxCtas);
   chpe::DeviceScope scope(c.device);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (cache_dtype == CHPE_F16) e = dtype == CHPE_F32 ? launch_d<__half, float>(P, head_dim, c.device, s)
-                                                     : launch_d<__half, __half>(P, head_dim, c.device, s);
-  else e = dtype == CHPE_F32 ? launch_d<__nv_bfloat16, float>(P, head_dim, c.device, s)
-                             : launch_d<__nv_bfloat16, __nv_bfloat16>(P, head_dim, c.device, s);
+  if (cache_dtype == CHPE_F16) e = dtype == CHPE_F32 ? launch_d<__half, float>(P, workspace, head_dim, c.device, s)
+                                                     : launch_d<__half, __half>(P, workspace, head_dim, c.device, s);
+  else e = dtype == CHPE_F32 ? launch_d<__nv_bfloat16, float>(P, workspace, head_dim, c.device, s)
+                             : launch_d<__nv_bfloat16, __nv_bfloat16>(P, workspace, head_dim, c.device, s);
   if (e != cudaSuccess) {
     snprintf(c.msg, sizeof(c.msg), "launch: %s", cudaGetErrorString(e));
     c.rc = -3;

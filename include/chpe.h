@@ -366,7 +366,7 @@ int chpe_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, in
  * t < seq_lens[b] (the new token's own among them: append it first), query
  * heads h*G .. h*G+G-1 on kv head h, G = num_heads / num_kv_heads of any size.
  * q and out [batch][num_heads][head_dim] of dtype, rows q_stride / out_stride
- * apart (q rows multiples of 16 bytes); out must not overlap q or the cache.
+ * apart (multiples of 16 bytes); out must not overlap q or the cache.
  * page_table: rows of max_pages entries, table_stride apart (0: one row for all);
  * entry p of a row is the page of positions p*page_size ..; page_size a power of
  * two from 16 to 65536.  Sequences may share pages.  seq_lens [batch] int32; a
