@@ -60,15 +60,15 @@ struct PagedLaunch {
   int64_t table_stride;
   const int32_t* lens;
   uint32_t n_pages, page_shift;
-  int64_t cap;  // positions a table row can hold
+  int32_t cap;  // positions a table row can hold
   int32_t B, H, KV, G, HT;  // HT: virtual heads (of up to 8 query heads) per kv head
   int32_t HW, groups;       // virtual heads of a CTA (a power of two); groups of them
-  int32_t tile;             // positions of a tile: 16 for each warp that shares a head
+  int32_t tile_shift;       // log2 of a tile's positions: 16 for each warp that shares a head
   float scale;
   void* out;
   int64_t out_stride;
   float* lse;
-  float* part;  // records [2 * grid][HW][8][D + 2]
+  float* part;  // records [2 * grid][HW]
   int4* desc;   // cuts: sequence, group, number of CTAs (0: not cut), the first of them
   int32_t by_seq;  // a desc entry for each sequence and group (they are at most `grid`); else for each CTA
 };
@@ -158,9 +158,9 @@ CHPE_DEV void store1(T* p, float v) {
 
 CHPE_DEV int seq_len(const PagedLaunch& P, int b) {
   const int n = P.lens[b];
-  return n <= 0 ? 0 : (int)min((int64_t)n, P.cap);
+  return max(0, min(n, P.cap));
 }
-CHPE_DEV int tiles_of(const PagedLaunch& P, int len) { return len / P.tile + (len % P.tile != 0); }
+CHPE_DEV int tiles_of(const PagedLaunch& P, int len) { return (len + (1 << P.tile_shift) - 1) >> P.tile_shift; }
 
 template <int D>
 struct Cfg {
@@ -169,8 +169,31 @@ struct Cfg {
   static constexpr int kStageBytes = 2 * kUnit * kRow;  // K and V of one unit
   static constexpr int kStages = 3;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kRec = D + 2;                    // floats of a record of one head: values, max, sum
+  static constexpr int kSums = D * 8 + 64;              // floats that a warp hands to another of its head
+  static constexpr int kRec = kHeads * (D + 2);         // floats of a warp's record: values, then (max, sum) of each head
   static constexpr int kMaxCtas = D == 64 ? 320 : 160;  // grid limit, sizes the workspace
+};
+
+// A place on the line of tiles, and the stretch of one sequence's group that
+// begins there.
+struct Cursor {
+  int t;        // next tile of the line
+  int b, base;  // sequence, its first tile
+  int group, tile0, n_tiles, tiles, len;
+
+  CHPE_DEV bool next(const PagedLaunch& P, int t_end) {
+    if (t >= t_end) return false;
+    while (t >= base + tiles * P.groups) {  // the next sequence that has tiles
+      base += tiles * P.groups;
+      len = seq_len(P, ++b);
+      tiles = tiles_of(P, len);
+    }
+    group = P.groups == 1 ? 0 : (int)((uint32_t)(t - base) / (uint32_t)tiles);
+    tile0 = t - base - group * tiles;
+    n_tiles = min(tiles - tile0, t_end - t);
+    t += n_tiles;
+    return true;
+  }
 };
 
 // T: type of the cache; TQ: of q and out.  Float queries over a BF16 cache take two
@@ -178,47 +201,44 @@ struct Cfg {
 template <typename T, typename TQ, int D>
 __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
+  constexpr bool SAME = std::is_same<T, TQ>::value;  // the query is its own only part
   constexpr int NP = std::is_same<T, __nv_bfloat16>::value && std::is_same<TQ, float>::value ? 2 : 1;
   constexpr int KS = D / 16, NT = D / 8, CH = D / 8;  // k steps, output n-tiles, 16-byte chunks per row
   constexpr int W = C::kWarps, THREADS = 32 * W;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long strip_sum[W];
-  __shared__ long long s_base;
-  __shared__ int s_seq;
+  __shared__ int strip_sum[W];
+  __shared__ int s_base, s_seq;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = lane >> 2, quad = lane & 3;
   const int cta = blockIdx.x, n_cta = gridDim.x;
-  const int hw = warp & (P.HW - 1), sub = warp / P.HW, subs = W / P.HW;
+  const int hw = warp & (P.HW - 1), sub = warp >> (31 - __clz(P.HW)), subs = 1 << (P.tile_shift - 4);
 
   // ---- this CTA's stretch of the line of tiles
   const int per = (P.B + THREADS - 1) / THREADS;
   const int b_lo = min(tid * per, P.B), b_hi = min(b_lo + per, P.B);
-  long long mine = 0;
+  int mine = 0;
   for (int b = b_lo; b < b_hi; b++) mine += tiles_of(P, seq_len(P, b));
   mine *= P.groups;
-  long long incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += up;
   }
   if (lane == 31) strip_sum[warp] = incl;
   __syncthreads();
-  long long before = 0, total = 0;
+  int total = 0;
 #pragma unroll
   for (int w = 0; w < W; w++) {
-    before += w < warp ? strip_sum[w] : 0;
+    incl += w < warp ? strip_sum[w] : 0;
     total += strip_sum[w];
   }
-  incl += before;
-  const long long share = total / n_cta, more = total % n_cta;
-  const long long t_begin = cta * share + min((long long)cta, more);
-  const long long t_end = t_begin + share + (cta < more ? 1 : 0);
+  const int share = (int)((uint32_t)total / (uint32_t)n_cta), more = total - share * n_cta;
+  const int t_begin = cta * share + min(cta, more), t_end = t_begin + share + (cta < more ? 1 : 0);
   if (t_begin < t_end && t_begin >= incl - mine && t_begin < incl) {  // one thread
-    long long base = incl - mine;
-    int b = b_lo;
+    int base = incl - mine, b = b_lo;
     for (; b < b_hi - 1; b++) {
-      const long long n = (long long)tiles_of(P, seq_len(P, b)) * P.groups;
+      const int n = tiles_of(P, seq_len(P, b)) * P.groups;
       if (t_begin < base + n) break;
       base += n;
     }
@@ -241,120 +261,136 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
     if (tid == 0 && !P.by_seq) P.desc[cta] = cut;
     return;
   }
-  int b = s_seq;
-  long long base = s_base;
-  int len = seq_len(P, b), tiles = tiles_of(P, len);
+  Cursor at;  // the stretch that is worked on
+  at.t = t_begin, at.b = s_seq, at.base = s_base;
+  at.len = seq_len(P, at.b), at.tiles = tiles_of(P, at.len);
 
   const uint32_t ring = smem_u32(smem) + warp * (C::kStages * C::kStageBytes);
   const size_t row_stride = (size_t)P.KV * D;  // elements between positions
   const T* const kc = static_cast<const T*>(P.kc);
   const T* const vc = static_cast<const T*>(P.vc);
 
-  for (long long t = t_begin; t < t_end;) {
-    while (t >= base + (long long)tiles * P.groups) {  // the next sequence that has tiles
-      base += (long long)tiles * P.groups;
-      len = seq_len(P, ++b);
-      tiles = tiles_of(P, len);
-    }
-    const int group = (int)((t - base) / tiles), tile0 = (int)((t - base) % tiles);
-    const int n_tiles = (int)min((long long)(tiles - tile0), t_end - t);
-    const int vh = group * P.HW + hw, kvh = vh / P.HT, h0 = kvh * P.G + (vh % P.HT) * kHeads;
-    const int nh = min(kHeads, (kvh + 1) * P.G - h0);
-    const int p0 = tile0 * P.tile + sub * kUnit;  // this warp's first unit
-
-    // ---- issue of one unit: rows [p, p+16) of this warp
-    const int32_t* const trow = P.table + b * P.table_stride;
-    int page_at = -1, page_val = 0;
-    auto page_of = [&](int it) {  // page of unit `it`; lanes hold 32 units' pages at a time
-      if ((it & ~31) != page_at) {
-        page_at = it & ~31;
-        const int64_t p = p0 + (int64_t)(page_at + lane) * P.tile;
-        page_val = p < len ? trow[p >> P.page_shift] : -1;
+  // ---- the units this warp will come to, copied kStages - 1 ahead across the
+  // ends of stretches: one step each time, one group of copies per step
+  Cursor ahead = at;
+  bool some = ahead.next(P, t_end);
+  int a_it = 0, a_st = 0, a_p = 0, page_val = -1;
+  const int32_t* a_row = nullptr;
+  size_t a_head = 0;
+  uint32_t ok_bits = 0;  // by stage: the unit's page is there
+  auto step_ahead = [&] {
+    if (some) {
+      if (a_it == 0) {
+        a_row = P.table + ahead.b * P.table_stride;
+        a_head = (size_t)((ahead.group * P.HW + hw) / P.HT) * D;
+        a_p = (ahead.tile0 << P.tile_shift) + sub * kUnit;
       }
-      const int pg = __shfl_sync(0xffffffffu, page_val, it & 31);
-      return (uint32_t)pg < P.n_pages ? pg : -1;
-    };
-    uint32_t ok_bits = 0;  // by stage: the unit's page is valid
-    auto issue = [&](int it) {
-      if (it < n_tiles) {
-        const int p = p0 + it * P.tile;
-        const int pg = page_of(it);
-        const int st = it % C::kStages;
-        ok_bits = (ok_bits & ~(1u << st)) | ((pg >= 0 ? 1u : 0u) << st);
-        const size_t r0 = ((size_t)(pg < 0 ? 0 : pg) << P.page_shift) + (p & ((1 << P.page_shift) - 1));
-        const T* const ks = kc + r0 * row_stride + (size_t)kvh * D;
-        const T* const vs = vc + r0 * row_stride + (size_t)kvh * D;
-        const uint32_t dst = ring + st * C::kStageBytes;
-        // a warp's instruction copies RPI rows; lane: row `hi` of them, chunk `ch`
-        constexpr int RPI = 32 / CH;
-        const int hi = lane / CH, ch = lane % CH;
+      if ((a_it & 31) == 0) {  // lanes hold 32 units' pages at a time
+        const int64_t p = a_p + ((int64_t)lane << P.tile_shift);
+        page_val = p < ahead.len ? a_row[p >> P.page_shift] : -1;
+      }
+      const int pg = __shfl_sync(0xffffffffu, page_val, a_it & 31);
+      const bool there = (uint32_t)pg < P.n_pages;
+      ok_bits = (ok_bits & ~(1u << a_st)) | ((there ? 1u : 0u) << a_st);
+      const size_t r0 = ((size_t)(there ? pg : 0) << P.page_shift) + (a_p & ((1 << P.page_shift) - 1));
+      const uint32_t dst = ring + a_st * C::kStageBytes;
+      // a warp's instruction copies RPI rows; lane: row `hi` of them, chunk `ch`
+      constexpr int RPI = 32 / CH;
+      const int hi = lane / CH, ch = lane % CH;
+      const T* k_at = kc + (r0 + hi) * row_stride + a_head + ch * 8;
+      const T* v_at = vc + (r0 + hi) * row_stride + a_head + ch * 8;
+      if (there && a_p + kUnit <= ahead.len) {
         const uint32_t d0 = dst + hi * C::kRow;
-        const T* k_at = ks + hi * row_stride + ch * 8;
-        const T* v_at = vs + hi * row_stride + ch * 8;
-        if (pg >= 0 && p + kUnit <= len) {
 #pragma unroll
-          for (int i = 0; i < kUnit / RPI; i++) {
-            const uint32_t d = d0 + i * RPI * C::kRow + (((ch ^ hi) ^ ((i * RPI) & 7)) << 4);
-            cp16(d, k_at);
-            cp16(d + kUnit * C::kRow, v_at);
-            k_at += RPI * row_stride;
-            v_at += RPI * row_stride;
-          }
-        } else {  // the sequence ends in this unit, or its page is not there: zeros
+        for (int i = 0; i < kUnit / RPI; i++) {
+          const uint32_t d = d0 + i * RPI * C::kRow + (((ch ^ hi) ^ ((i * RPI) & 7)) << 4);
+          cp16(d, k_at);
+          cp16(d + kUnit * C::kRow, v_at);
+          k_at += RPI * row_stride;
+          v_at += RPI * row_stride;
+        }
+      } else {  // the sequence ends in this unit, or its page is not there: zeros
 #pragma unroll 1
-          for (int i = 0; i < kUnit / RPI; i++) {
-            const int r = i * RPI + hi;
-            const bool on = pg >= 0 && p + r < len;
-            const uint32_t d = dst + r * C::kRow + ((ch ^ (r & 7)) << 4);
-            cp16_if(d, on ? k_at + i * RPI * row_stride : kc, on);
-            cp16_if(d + kUnit * C::kRow, on ? v_at + i * RPI * row_stride : vc, on);
-          }
+        for (int i = 0; i < kUnit / RPI; i++) {
+          const int r = i * RPI + hi;
+          const bool on = there && a_p + r < ahead.len;
+          const uint32_t d = dst + r * C::kRow + ((ch ^ (r & 7)) << 4);
+          cp16_if(d, on ? k_at + i * RPI * row_stride : kc, on);
+          cp16_if(d + kUnit * C::kRow, on ? v_at + i * RPI * row_stride : vc, on);
         }
       }
-      cp_commit();
-    };
-#pragma unroll
-    for (int s = 0; s < C::kStages - 1; s++) issue(s);
+      a_st = a_st + 1 < C::kStages ? a_st + 1 : 0;
+      a_p += 1 << P.tile_shift;
+      if (++a_it == ahead.n_tiles) {
+        a_it = 0;
+        some = ahead.next(P, t_end);
+      }
+    }
+    cp_commit();
+  };
+  int st = 0;  // stage of the unit that is worked on
+  bool started = false;
+
+  while (at.next(P, t_end)) {
+    const int vh = at.group * P.HW + hw, kvh = vh / P.HT, h0 = kvh * P.G + (vh % P.HT) * kHeads;
+    const int nh = min(kHeads, (kvh + 1) * P.G - h0);
 
     // ---- the query's parts as A operands: rows 0-7 hi, 8-15 lo
     uint32_t qa[NP][KS][4];
-    float q_scale;  // back from the scaled parts, times scale * log2(e)
+    float q_scale = P.scale * 1.44269504088896340736f;  // scores in powers of two
     {
+      const TQ* const q_row = static_cast<const TQ*>(P.q) + at.b * P.q_stride + (int64_t)(h0 + row) * D + 2 * quad;
+      if constexpr (SAME) {
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            qa[0][k][2 * h] = row < nh ? *reinterpret_cast<const uint32_t*>(q_row + k * 16 + h * 8) : 0u;
+            qa[0][k][2 * h + 1] = 0u;
+          }
+      }
       float2 x[KS][2];
-      float top = 0.f;
-      const TQ* const q_row = static_cast<const TQ*>(P.q) + b * P.q_stride + (int64_t)(h0 + row) * D + 2 * quad;
+      if constexpr (!SAME) {
 #pragma unroll
-      for (int k = 0; k < KS; k++)
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          x[k][h] = row < nh ? load2(q_row + k * 16 + h * 8) : make_float2(0.f, 0.f);
-          top = fmaxf(top, fmaxf(fabsf(x[k][h].x), fabsf(x[k][h].y)));
-        }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // a power of two that brings the largest |q| of the head to [1, 2): FP16
-      // parts neither overflow nor lose small heads
-      int e = 0;
-      if (top > 0.f && top < INFINITY) e = ilogbf(top);
-      e = max(-126, min(126, e));
-      const float down = ldexpf(1.f, -e);
-      q_scale = P.scale * 1.44269504088896340736f * ldexpf(1.f, e);
+          for (int h = 0; h < 2; h++) x[k][h] = row < nh ? load2(q_row + k * 16 + h * 8) : make_float2(0.f, 0.f);
+      }
+      if (!started) {  // the first copies, behind the query's loads
+#pragma unroll 1
+        for (int i = 0; i < C::kStages - 1; i++) step_ahead();
+        started = true;
+      }
+      if constexpr (!SAME) {
+        float top = 0.f;
 #pragma unroll
-      for (int k = 0; k < KS; k++)
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float2 y = make_float2(x[k][h].x * down, x[k][h].y * down);
+          for (int h = 0; h < 2; h++) top = fmaxf(top, fmaxf(fabsf(x[k][h].x), fabsf(x[k][h].y)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // a power of two that brings the largest |q| of the head to [1, 2): FP16 parts
+        // neither overflow nor lose small heads
+        const int e = top < INFINITY ? max(-126, min(126, (int)(__float_as_uint(top) >> 23) - 127)) : 0;
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        q_scale *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-          for (int np = 0; np < NP; np++)
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-            for (int part = 0; part < 2; part++) {
-              const uint32_t w = pack2<T>(y.x, y.y);
-              qa[np][k][2 * h + part] = w;
-              const float2 f = unpack2<T>(w);
-              y.x -= f.x;
-              y.y -= f.y;
-            }
-        }
+          for (int h = 0; h < 2; h++) {
+            float2 y = make_float2(x[k][h].x * down, x[k][h].y * down);
+#pragma unroll
+            for (int np = 0; np < NP; np++)
+#pragma unroll
+              for (int part = 0; part < 2; part++) {
+                const uint32_t w = pack2<T>(y.x, y.y);
+                qa[np][k][2 * h + part] = w;
+                const float2 f = unpack2<T>(w);
+                y.x -= f.x;
+                y.y -= f.y;
+              }
+          }
+      }
     }
 
     float o[NT][4];
@@ -371,13 +407,12 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
     const int k_row = (mat >> 1) * 8 + mr, k_ch = mat & 1;
     const int v_row = (mat & 1) * 8 + mr, v_ch = mat >> 1;
 
-    for (int it = 0; it < n_tiles; it++) {
-      issue(it + C::kStages - 1);
+    int p = (at.tile0 << P.tile_shift) + sub * kUnit;
+    for (int it = 0; it < at.n_tiles; it++, p += 1 << P.tile_shift) {
+      step_ahead();
       cp_wait<C::kStages - 1>();
       __syncwarp();
-      const int st = it % C::kStages;
-      const int p = p0 + it * P.tile;
-      if (p < len && (ok_bits >> st & 1u)) {
+      if (p < at.len && (ok_bits >> st & 1u)) {
         const uint32_t kb = ring + st * C::kStageBytes, vb = kb + kUnit * C::kRow;
         float s[2][4] = {};
 #pragma unroll
@@ -396,7 +431,7 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
         for (int j = 0; j < 2; j++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const bool in = p + 8 * j + 2 * quad + e < len;
+            const bool in = p + 8 * j + 2 * quad + e < at.len;
             sc[j][e] = in ? (s[j][e] + s[j][e + 2]) * q_scale : -INFINITY;
             mx = fmaxf(mx, sc[j][e]);
           }
@@ -441,128 +476,170 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
         }
       }
       __syncwarp();  // the stage may be filled again
+      st = st + 1 < C::kStages ? st + 1 : 0;
     }
-    cp_wait<0>();
     if (subs > 1) {  // warps that share the head: the first one takes the others' sums
-      __syncthreads();  // every ring is drained: their memory holds the sums now
-      constexpr int kSums = NT * 64 + 64;  // floats of a warp: a pair per lane and n-tile, m and l
-      float* const mine_at = reinterpret_cast<float*>(smem) + (size_t)warp * kSums + 2 * lane;
+      float* const sums = reinterpret_cast<float*>(smem + C::kRing) + hw * C::kSums + 2 * lane;
+      __syncthreads();  // the sums of the stretch before are taken
       if (sub > 0) {
+        float* const to = sums + (sub - 1) * P.HW * C::kSums;  // a pair per lane and n-tile, then m and l
 #pragma unroll
         for (int n = 0; n < NT; n++)
-          *reinterpret_cast<float2*>(mine_at + n * 64) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
-        *reinterpret_cast<float2*>(mine_at + NT * 64) = make_float2(m, l);
+          *reinterpret_cast<float2*>(to + n * 64) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+        *reinterpret_cast<float2*>(to + NT * 64) = make_float2(m, l);
       }
       __syncthreads();
       if (sub == 0) {
-        for (int w = 1; w < subs; w++) {
-          const float* const at = mine_at + (size_t)w * P.HW * kSums;
-          const float2 ml = *reinterpret_cast<const float2*>(at + NT * 64);
+        for (int w = 0; w < subs - 1; w++) {
+          const float* const from = sums + w * P.HW * C::kSums;
+          const float2 ml = *reinterpret_cast<const float2*>(from + NT * 64);
           const float top = fmaxf(m, ml.x);
           const float fa = m == -INFINITY ? 0.f : exp2f(m - top), fb = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
           l = l * fa + ml.y * fb;
           m = top;
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            const float2 v = *reinterpret_cast<const float2*>(at + n * 64);
+            const float2 v = *reinterpret_cast<const float2*>(from + n * 64);
             o[n][0] = (o[n][0] + o[n][2]) * fa + v.x * fb;
             o[n][1] = (o[n][1] + o[n][3]) * fa + v.y * fb;
             o[n][2] = o[n][3] = 0.f;
           }
         }
       }
-      __syncthreads();  // the next stretch fills the rings again
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (sub == 0 && row < nh) {
-      if (n_tiles == tiles) {
+      if (at.n_tiles == at.tiles) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        TQ* const out = static_cast<TQ*>(P.out) + b * P.out_stride + (int64_t)(h0 + row) * D + 2 * quad;
+        TQ* const out = static_cast<TQ*>(P.out) + at.b * P.out_stride + (int64_t)(h0 + row) * D + 2 * quad;
 #pragma unroll
         for (int n = 0; n < NT; n++) store2(out + n * 8, (o[n][0] + o[n][2]) * inv, (o[n][1] + o[n][3]) * inv);
         if (P.lse && quad == 0)
-          P.lse[(int64_t)b * P.H + h0 + row] =
+          P.lse[(int64_t)at.b * P.H + h0 + row] =
               l == 0.f ? -INFINITY : 0.693147180559945309417f * (m + (log2f(l) - kPShift));
       } else {
         // hi and lo rows add up to the head's value
-        float* const rec = P.part + (((size_t)2 * cta + (tile0 == 0 ? 1 : 0)) * P.HW + hw) * kHeads * C::kRec +
-                           row * C::kRec + 2 * quad;
+        float* const rec = P.part + (((size_t)2 * cta + (at.tile0 == 0 ? 1 : 0)) * P.HW + hw) * C::kRec;
 #pragma unroll
         for (int n = 0; n < NT; n++)
-          *reinterpret_cast<float2*>(rec + n * 8) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
-        if (quad == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(m, l);
+          *reinterpret_cast<float2*>(rec + row * D + n * 8 + 2 * quad) =
+              make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+        if (quad == 0) *reinterpret_cast<float2*>(rec + kHeads * D + 2 * row) = make_float2(m, l);
       }
     }
-    if (tile0 == 0) {
+    if (at.tile0 == 0) {
       cut = make_int4(0, 0, 0, 0);
-      if (n_tiles < tiles) {  // the CTAs that hold the rest of the group's tiles follow without a gap
-        const long long last = base + (long long)(group + 1) * tiles - 1;
-        const long long big = (share + 1) * more;  // tiles of the CTAs with one more
-        const long long owner = last < big ? last / (share + 1) : more + (last - big) / share;
-        cut = make_int4(b, group, (int)(owner - cta) + 1, cta);
+      if (at.n_tiles < at.tiles) {  // the CTAs that hold the rest of the group's tiles follow without a gap
+        const int last = at.base + (at.group + 1) * at.tiles - 1;
+        const int big = (share + 1) * more;  // tiles of the CTAs with one more
+        const int owner = last < big ? last / (share + 1) : more + (last - big) / share;
+        cut = make_int4(at.b, at.group, owner - cta + 1, cta);
       }
-      if (tid == 0 && P.by_seq) P.desc[b * P.groups + group] = cut;
+      if (tid == 0 && P.by_seq) P.desc[at.b * P.groups + at.group] = cut;
     }
-    t += n_tiles;
   }
   if (tid == 0 && !P.by_seq) P.desc[cta] = cut;
 }
 
 // Joins the records of a cut group: blockIdx.x the desc entry, blockIdx.y the
-// query head within the group.
-template <typename TQ, int D>
-__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ PagedLaunch P) {
+// query head within the group.  The records' weights are worked out once, side by
+// side, then each warp adds up every kJoinWarps-th record, kBatch loads at a time (148 records
+// of 128 values, one per SM: 4 us; one by one with their weights they took 22).
+template <typename TQ, int D, int kJoinWarps>
+__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
-  constexpr int PER = D / 64;  // pairs per lane
-  __shared__ float sv[4][D], sl[4];
+  constexpr int V = D > 128 ? D / 128 : 1, LANES = D / 4 < 32 ? D / 4 : 32;  // float4s per lane, lanes of a record
+  constexpr int kBatch = 8;
+  __shared__ float weight[C::kMaxCtas];
+  __shared__ float sv[kJoinWarps][D];
+  __shared__ float red[2][kJoinWarps];
   pdl_wait();
   const int4 cut = P.desc[blockIdx.x];
-  const int n = cut.z;
+  const int n = cut.z;  // at most one record per CTA
   if (n == 0) return;
   const int hw = blockIdx.y / kHeads, h = blockIdx.y % kHeads, vh = cut.y * P.HW + hw;
   const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * kHeads + h;
   if (head >= (kvh + 1) * P.G) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // record i: the beginning lies in slot 1 of the first CTA, the others in slot 0 of theirs
-  auto rec = [&](int i) {
-    return P.part + (((size_t)2 * (cut.w + i) + (i == 0 ? 1 : 0)) * P.HW + hw) * kHeads * C::kRec + h * C::kRec;
-  };
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, rec(i)[D]);
-  M = warp_max(M);
-  float2 v[PER] = {};
-  float L = 0.f;
-#pragma unroll 8
-  for (int i = warp; i < n; i += 4) {
-    const float* r = rec(i);
-    const float2 ml = *reinterpret_cast<const float2*>(r + D);
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-    L = fmaf(ml.y, w, L);
+  auto rec = [&](int i) { return P.part + (((size_t)2 * (cut.w + i) + (i == 0 ? 1 : 0)) * P.HW + hw) * C::kRec; };
+  auto fetch = [&](float4 (&x)[V], int i) {
 #pragma unroll
-    for (int e = 0; e < PER; e++) {
-      const float2 x = *reinterpret_cast<const float2*>(r + 64 * e + 2 * lane);
-      v[e].x = fmaf(x.x, w, v[e].x);
-      v[e].y = fmaf(x.y, w, v[e].y);
+    for (int e = 0; e < V; e++)
+      x[e] = i < n && lane < LANES ? *reinterpret_cast<const float4*>(rec(i) + h * D + 128 * e + 4 * lane)
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  float4 x[kBatch][V];
+#pragma unroll
+  for (int j = 0; j < kBatch; j++) fetch(x[j], warp + j * kJoinWarps);
+
+  constexpr int PER = (C::kMaxCtas + 32 * kJoinWarps - 1) / (32 * kJoinWarps);
+  float2 ml[PER];
+  float M = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int i = tid + j * 32 * kJoinWarps;
+    ml[j] = i < n ? *reinterpret_cast<const float2*>(rec(i) + kHeads * D + 2 * h) : make_float2(-INFINITY, 0.f);
+    M = fmaxf(M, ml[j].x);
+  }
+  M = warp_max(M);
+  if (lane == 0) red[0][warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; w++) M = fmaxf(M, red[0][w]);
+  float L = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int i = tid + j * 32 * kJoinWarps;
+    const float w = ml[j].x == -INFINITY ? 0.f : exp2f(ml[j].x - M);
+    if (i < n) weight[i] = w;
+    L = fmaf(ml[j].y, w, L);  // a NaN sum stays
+  }
+  L = warp_sum(L);
+  if (lane == 0) red[1][warp] = L;
+  __syncthreads();
+  L = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; w++) L += red[1][w];
+
+  float4 v[V];
+#pragma unroll
+  for (int e = 0; e < V; e++) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = warp; i0 < n; i0 += kBatch * kJoinWarps) {
+#pragma unroll
+    for (int j = 0; j < kBatch; j++) {
+      const int i = i0 + j * kJoinWarps;
+      if (i >= n) break;
+      const float w = weight[i];
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        v[e].x = fmaf(x[j][e].x, w, v[e].x);
+        v[e].y = fmaf(x[j][e].y, w, v[e].y);
+        v[e].z = fmaf(x[j][e].z, w, v[e].z);
+        v[e].w = fmaf(x[j][e].w, w, v[e].w);
+      }
+      fetch(x[j], i + kBatch * kJoinWarps);
     }
   }
+  if (lane < LANES)
 #pragma unroll
-  for (int e = 0; e < PER; e++) *reinterpret_cast<float2*>(&sv[warp][64 * e + 2 * lane]) = v[e];
-  if (lane == 0) sl[warp] = L;
+    for (int e = 0; e < V; e++) *reinterpret_cast<float4*>(&sv[warp][128 * e + 4 * lane]) = v[e];
   __syncthreads();
-  L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  for (int d = threadIdx.x; d < D; d += 128) {
-    const float x = (sv[0][d] + sv[1][d]) + (sv[2][d] + sv[3][d]);
-    store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)head * D + d, L == 0.f ? 0.f : x / L);
+  for (int d = tid; d < D; d += 32 * kJoinWarps) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; w++) y += sv[w][d];
+    store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)head * D + d, L == 0.f ? 0.f : y / L);
   }
-  if (P.lse && threadIdx.x == 0)
+  if (P.lse && tid == 0)
     P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
 }
 
 template <int D>
 constexpr size_t workspace_bytes_of() {
   using C = Cfg<D>;
-  return C::kMaxCtas * sizeof(int4) + (size_t)2 * C::kMaxCtas * C::kWarps * kHeads * C::kRec * sizeof(float);
+  return C::kMaxCtas * sizeof(int4) + (size_t)2 * C::kMaxCtas * C::kWarps * C::kRec * sizeof(float);
 }
 
 template <typename T, typename TQ, int D>
@@ -574,36 +651,40 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   int grid = dev >= 0 ? __atomic_load_n(&grid_of[dev], __ATOMIC_RELAXED) : 0;
   if (grid == 0) {
     int sms = 0, res = 0;
-    cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, TQ, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing);
+    const int most = C::kRing + (C::kWarps - 1) * C::kSums * (int)sizeof(float);  // one head: all other warps hand over
+    cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, TQ, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess)
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, TQ, D>, 32 * C::kWarps, C::kRing);
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, TQ, D>, 32 * C::kWarps, most);
     if (e != cudaSuccess) return e;
     grid = sms * (res < 1 ? 1 : res);
     if (grid > C::kMaxCtas) grid = C::kMaxCtas;
     if (dev >= 0) __atomic_store_n(&grid_of[dev], grid, __ATOMIC_RELAXED);
   }
-  const int vh = P.KV * P.HT;
-  P.HW = C::kWarps;
-  while (vh % P.HW != 0) P.HW /= 2;
-  P.groups = vh / P.HW;
-  P.tile = kUnit * (C::kWarps / P.HW);
+  const int subs = C::kWarps / P.HW;
   P.by_seq = (int64_t)P.B * P.groups <= grid;
   P.desc = static_cast<int4*>(workspace);
   P.part = reinterpret_cast<float*>(P.desc + C::kMaxCtas);
-  paged_kernel<T, TQ, D><<<grid, 32 * C::kWarps, C::kRing, s>>>(P);
-  cudaError_t e = cudaGetLastError();
+  paged_kernel<T, TQ, D><<<grid, 32 * C::kWarps, C::kRing + (subs - 1) * P.HW * C::kSums * sizeof(float), s>>>(P);
+  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(P.by_seq ? P.B * P.groups : grid, P.HW * kHeads);
-  cfg.blockDim = dim3(128);
-  cfg.stream = s;
+  // started while the kernel above ends; it waits for it before it reads anything
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D>, P);
+  const int cuts = P.by_seq ? P.B * P.groups : grid;
+  cfg.gridDim = dim3(cuts, P.HW * kHeads);
+  // few groups: cut into many records each; many groups: into two or three
+  if (cuts * 8 <= grid) {
+    cfg.blockDim = dim3(32 * 8);
+    return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, 8>, P);
+  }
+  cfg.blockDim = dim3(32 * 2);
+  return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, 2>, P);
 }
 
 template <typename T, typename TQ>
@@ -674,11 +755,20 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   P.table = page_table, P.table_stride = table_stride, P.lens = seq_lens;
   P.n_pages = num_pages;
   while ((1u << P.page_shift) < page_size) P.page_shift++;
-  P.cap = num_pages ? (int64_t)max_pages * page_size : 0;  // an empty pool holds no position
-  if (P.cap > INT32_MAX - 1024) P.cap = INT32_MAX - 1024;
+  const int64_t cap = num_pages ? (int64_t)max_pages * page_size : 0;  // an empty pool holds no position
+  P.cap = (int32_t)(cap < INT32_MAX - 1024 ? cap : INT32_MAX - 1024);
   P.B = (int32_t)batch, P.H = (int32_t)num_heads, P.KV = (int32_t)num_kv_heads;
   P.G = P.H / P.KV;
   P.HT = (P.G + kHeads - 1) / kHeads;
+  const int vh = P.KV * P.HT, warps = head_dim == 256 ? Cfg<256>::kWarps : Cfg<128>::kWarps;
+  static_assert(Cfg<64>::kWarps == Cfg<128>::kWarps, "");
+  P.HW = warps;
+  while (vh % P.HW != 0) P.HW /= 2;
+  P.groups = vh / P.HW;
+  P.tile_shift = 4;
+  while ((kUnit * warps / P.HW) >> P.tile_shift > 1) P.tile_shift++;
+  if ((int64_t)((P.cap >> P.tile_shift) + 1) * P.groups > INT32_MAX / P.B)
+    return c.fail(-1, "batch * max_pages * page_size is too large"), c.done();
   P.scale = scale;
   P.out = out, P.out_stride = out_stride, P.lse = lse;
   chpe::DeviceScope scope(c.device);
