@@ -10,8 +10,8 @@
 //
 // Work split.  A CTA takes several kv heads of the same positions at once, a warp
 // each, because a position's heads lie side by side in the cache: what a CTA reads
-// is then whole pages, not a 256-byte row of every 2 KB (one head per CTA, all else
-// alike: 162 us instead of @FULL for a batch of 64 on 64/8 heads of 128).  Where there are
+// is then whole pages, not a 256-byte row of every 2 KB (one head per CTA
+// took 162 us instead of 124 for a batch of 64 on 64/8 heads of 128).  Where there are
 // fewer heads than warps the remaining warps take further 16-position units of
 // the tile.  The work is a line of tiles: sequence by sequence, group of heads by
 // group, tile by tile, and CTA c of C takes the c-th of C equal stretches,
@@ -24,9 +24,17 @@
 // not depend on timing.
 //
 // Each warp has a ring of its own in shared memory (cp.async, 16-byte chunks
-// XOR-swizzled by row so that ldmatrix is free of bank conflicts), a running
-// maximum and sums in registers, and waits for no other warp; only warps that
-// share a head meet, at the end of a stretch.
+// XOR-swizzled by row so that ldmatrix is free of bank conflicts) that runs
+// ahead across the ends of sequences, a running maximum and sums in registers, and
+// waits for no other warp; only warps that share a head meet, at the end of a part.
+//
+// Measured (device time): 131071 positions of one sequence on 64/8 heads of 128: 92 us,
+// 90 % of the copy rate; 64 sequences of up to 8192 there: 124 us, 90 %; 37 of up
+// to 4093 on 16/4 heads of 256: 52 us, 62 %; one of 77 on 16/2 heads: 7.6 us.
+// What is left: SMs get bandwidth unevenly, so that CTAs with equal shares end
+// 10 % before and after the mean, and the records' join, 3 us behind a gap of 2.
+// Handing a fifth of the line out to whoever is done evened the ends out but cost as
+// much in more, shorter parts.
 //
 // Matrix instructions: mma.sync m16n8k16.  A batch-1 product has 8 query heads
 // at most per tile against 16 rows of the instruction; the spare 8 rows carry the low
@@ -543,43 +551,43 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
 }
 
 // Joins the records of a cut group: blockIdx.x the desc entry, blockIdx.y the
-// query head within the group.  The records' weights are worked out once, side by
-// side, then each warp adds up every kJoinWarps-th record, kBatch loads at a time (148 records
-// of 128 values, one per SM: 4 us; one by one with their weights they took 22).
-template <typename TQ, int D, int kJoinWarps>
-__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ PagedLaunch P) {
+// query head within the group and the DB of its D values.  The records' weights
+// are worked out once, side by side; 4 * DB bytes of a record take DB/4 lanes, and every
+// lane has kBatch records' loads in flight.
+template <typename TQ, int D, int DB, int JW>
+__global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D>;
-  constexpr int V = D > 128 ? D / 128 : 1, LANES = D / 4 < 32 ? D / 4 : 32;  // float4s per lane, lanes of a record
-  constexpr int kBatch = 8;
-  __shared__ float weight[C::kMaxCtas];
-  __shared__ float sv[kJoinWarps][D];
-  __shared__ float red[2][kJoinWarps];
+  constexpr int kLanes = DB / 4, kRows = 32 * JW / kLanes;  // lanes of a record, records side by side
+  constexpr int kBatch = 8, kMax = C::kMaxCtas;
+  static_assert(32 * JW % kLanes == 0, "");
+  __shared__ float weight[kMax];
+  __shared__ float sv[kRows][DB];
+  __shared__ float red[2][JW];
   pdl_wait();
   const int4 cut = P.desc[blockIdx.x];
   const int n = cut.z;  // at most one record per CTA
   if (n == 0) return;
-  const int hw = blockIdx.y / kHeads, h = blockIdx.y % kHeads, vh = cut.y * P.HW + hw;
+  const int slice = blockIdx.y % (D / DB), hh = blockIdx.y / (D / DB);
+  const int hw = hh / kHeads, h = hh % kHeads, vh = cut.y * P.HW + hw;
   const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * kHeads + h;
   if (head >= (kvh + 1) * P.G) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int my_row = tid / kLanes, col = slice * DB + 4 * (tid % kLanes);
   // record i: the beginning lies in slot 1 of the first CTA, the others in slot 0 of theirs
   auto rec = [&](int i) { return P.part + (((size_t)2 * (cut.w + i) + (i == 0 ? 1 : 0)) * P.HW + hw) * C::kRec; };
-  auto fetch = [&](float4 (&x)[V], int i) {
-#pragma unroll
-    for (int e = 0; e < V; e++)
-      x[e] = i < n && lane < LANES ? *reinterpret_cast<const float4*>(rec(i) + h * D + 128 * e + 4 * lane)
-                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 x[kBatch];
+  auto fetch = [&](int j, int i) {
+    x[j] = i < n ? *reinterpret_cast<const float4*>(rec(i) + h * D + col) : make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  float4 x[kBatch][V];
 #pragma unroll
-  for (int j = 0; j < kBatch; j++) fetch(x[j], warp + j * kJoinWarps);
+  for (int j = 0; j < kBatch; j++) fetch(j, my_row + j * kRows);
 
-  constexpr int PER = (C::kMaxCtas + 32 * kJoinWarps - 1) / (32 * kJoinWarps);
+  constexpr int PER = (kMax + 32 * JW - 1) / (32 * JW);
   float2 ml[PER];
   float M = -INFINITY;
 #pragma unroll
   for (int j = 0; j < PER; j++) {
-    const int i = tid + j * 32 * kJoinWarps;
+    const int i = tid + j * 32 * JW;
     ml[j] = i < n ? *reinterpret_cast<const float2*>(rec(i) + kHeads * D + 2 * h) : make_float2(-INFINITY, 0.f);
     M = fmaxf(M, ml[j].x);
   }
@@ -587,11 +595,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
   if (lane == 0) red[0][warp] = M;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; w++) M = fmaxf(M, red[0][w]);
+  for (int w = 0; w < JW; w++) M = fmaxf(M, red[0][w]);
   float L = 0.f;
 #pragma unroll
   for (int j = 0; j < PER; j++) {
-    const int i = tid + j * 32 * kJoinWarps;
+    const int i = tid + j * 32 * JW;
     const float w = ml[j].x == -INFINITY ? 0.f : exp2f(ml[j].x - M);
     if (i < n) weight[i] = w;
     L = fmaf(ml[j].y, w, L);  // a NaN sum stays
@@ -601,38 +609,30 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
   __syncthreads();
   L = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; w++) L += red[1][w];
+  for (int w = 0; w < JW; w++) L += red[1][w];
 
-  float4 v[V];
-#pragma unroll
-  for (int e = 0; e < V; e++) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = warp; i0 < n; i0 += kBatch * kJoinWarps) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = my_row; i0 < n; i0 += kBatch * kRows) {
 #pragma unroll
     for (int j = 0; j < kBatch; j++) {
-      const int i = i0 + j * kJoinWarps;
+      const int i = i0 + j * kRows;
       if (i >= n) break;
       const float w = weight[i];
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        v[e].x = fmaf(x[j][e].x, w, v[e].x);
-        v[e].y = fmaf(x[j][e].y, w, v[e].y);
-        v[e].z = fmaf(x[j][e].z, w, v[e].z);
-        v[e].w = fmaf(x[j][e].w, w, v[e].w);
-      }
-      fetch(x[j], i + kBatch * kJoinWarps);
+      v.x = fmaf(x[j].x, w, v.x);
+      v.y = fmaf(x[j].y, w, v.y);
+      v.z = fmaf(x[j].z, w, v.z);
+      v.w = fmaf(x[j].w, w, v.w);
+      fetch(j, i + kBatch * kRows);
     }
   }
-  if (lane < LANES)
-#pragma unroll
-    for (int e = 0; e < V; e++) *reinterpret_cast<float4*>(&sv[warp][128 * e + 4 * lane]) = v[e];
+  *reinterpret_cast<float4*>(&sv[my_row][4 * (tid % kLanes)]) = v;
   __syncthreads();
-  for (int d = tid; d < D; d += 32 * kJoinWarps) {
+  for (int d = tid; d < DB; d += 32 * JW) {
     float y = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; w++) y += sv[w][d];
-    store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)head * D + d, L == 0.f ? 0.f : y / L);
+    for (int w = 0; w < min(n, kRows); w++) y += sv[w][d];
+    store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)head * D + slice * DB + d, L == 0.f ? 0.f : y / L);
   }
-  if (P.lse && tid == 0)
+  if (P.lse && tid == 0 && slice == 0)
     P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
 }
 
@@ -677,14 +677,18 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   const int cuts = P.by_seq ? P.B * P.groups : grid;
-  cfg.gridDim = dim3(cuts, P.HW * kHeads);
-  // few groups: cut into many records each; many groups: into two or three
-  if (cuts * 8 <= grid) {
-    cfg.blockDim = dim3(32 * 8);
-    return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, 8>, P);
+  // The records that a group may be cut into: many are joined by many threads (one
+  // sequence of 8192 on 64/8 heads: 16.0 us, with two warps per query head 20.2),
+  // few by two warps (16 sequences of 150 on 16/2 heads: 8.2 us, with 16 warps 11.0).
+  const int64_t records = (P.cap >> P.tile_shift) < grid / cuts + 2 ? (P.cap >> P.tile_shift) : grid / cuts + 2;
+  if (records > 16) {
+    cfg.gridDim = dim3(cuts, P.HW * kHeads * (D / 64));
+    cfg.blockDim = dim3(32 * 16);
+    return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, 64, 16>, P);
   }
+  cfg.gridDim = dim3(cuts, P.HW * kHeads);
   cfg.blockDim = dim3(32 * 2);
-  return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, 2>, P);
+  return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, D, 2>, P);
 }
 
 template <typename T, typename TQ>
