@@ -50,6 +50,7 @@ SYMBOLS = [
     ("chpe_convert_archive", _I, [C.c_char_p, C.c_char_p, _I, _I]),
     ("chpe_decode_step", _I, [_P, _U32, _U32, _FP]),
     ("chpe_generate", _I, [_P, _U32P, _S, _S, _U32P]),
+    ("chpe_generate_processed", _I, [_P, _U32P, _S, _S, _F, _F, _F, C.POINTER(C.c_int32), _FP, _S, _U32P, _U32P]),
     ("chpe_speculative_generate", _I, [_P, _U32P, _S, _S, _U32, _U32, _U32P, C.POINTER(C.c_uint64)]),
     ("chpe_bench_greedy", _I, [_P, _S, _FP]),
     ("chpe_bench_host", _I, [_P, _U32P, _S, _FP, C.POINTER(C.c_double)]),
@@ -328,6 +329,24 @@ class Engine:
         out = np.zeros(max(n_gen, 1), np.uint32)
         if lib().chpe_generate(self.ctx, _u32p(p), p.size, n_gen, _u32p(out)) != 0:
             raise ChpeError(self._err() or "chpe_generate failed")
+        return out[:n_gen]
+
+    def generate_processed(self, prompt, n_gen: int, repetition: float = 1.0, frequency: float = 0.0,
+                           presence: float = 0.0, bias: dict[int, float] | None = None, mask=None) -> np.ndarray:
+        """chpe_generate_processed: generate() under penalties, biases {token: value}
+        and a mask (ceil(vocab/32) words, bit 1: allowed)."""
+        p = np.ascontiguousarray(prompt, dtype=np.uint32)
+        ids = np.array(list(bias or {}), np.int32)
+        vals = np.array(list((bias or {}).values()), np.float32)
+        if mask is not None:
+            mask = np.ascontiguousarray(mask).view(np.uint32)
+            if mask.shape != ((self.vocab + 31) // 32,):
+                raise ValueError(f"mask must have {(self.vocab + 31) // 32} words")
+        out = np.zeros(max(n_gen, 1), np.uint32)
+        if lib().chpe_generate_processed(self.ctx, _u32p(p), p.size, n_gen, repetition, frequency, presence,
+                                         ids.ctypes.data_as(C.POINTER(C.c_int32)), _fp(vals), ids.size,
+                                         _u32p(mask) if mask is not None else None, _u32p(out)) != 0:
+            raise ChpeError(self._err() or "chpe_generate_processed failed")
         return out[:n_gen]
 
     def speculative_generate(self, prompt, n_gen: int, draft_len: int = 4,

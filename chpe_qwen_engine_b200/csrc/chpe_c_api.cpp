@@ -269,6 +269,22 @@ int chpe_generate(void* ctx, const uint32_t* prompt, size_t n_prompt, size_t n_g
   return 0;
 }
 
+int chpe_generate_processed(void* ctx, const uint32_t* prompt, size_t n_prompt, size_t n_gen, float repetition,
+                            float frequency, float presence, const int32_t* bias_ids, const float* bias_values,
+                            size_t n_bias, const uint32_t* mask, uint32_t* out) {
+  if (!ctx || !prompt || n_prompt == 0 || (n_gen > 0 && !out) || (n_bias > 0 && (!bias_ids || !bias_values))) return -1;
+  Ctx* c = (Ctx*)ctx;
+  try {
+    c->engine->generate_processed(prompt, n_prompt, n_gen, repetition, frequency, presence, bias_ids, bias_values,
+                                  n_bias, mask, out);
+    store_result(c);
+  } catch (const std::exception& e) {
+    c->err = e.what();
+    return -1;
+  }
+  return 0;
+}
+
 int chpe_speculative_generate(void* ctx, const uint32_t* prompt, size_t n_prompt, size_t n_gen,
                               uint32_t draft_len, uint32_t ngram, uint32_t* out, uint64_t* stats) {
   if (!ctx || !prompt || n_prompt == 0 || (n_gen > 0 && !out)) return -1;

@@ -13,6 +13,7 @@
 #include <string>
 #include <vector>
 
+#include "../../include/chpe.h"
 #include "attention.cuh"
 #include "aux_kernels.cuh"
 #include "gemv.cuh"
@@ -1882,6 +1883,89 @@ void Engine::generate(const uint32_t* prompt, size_t n_prompt, size_t n_gen, uin
   sync_result();
   for (size_t i = 1; i < n_gen; i++) out_tokens[i] = (uint32_t)g[i - 1];
   pos_ = (uint32_t)(n_prompt + n_gen - 1);
+}
+
+// Takes the token that the rules chose: into the history (whose length grows by
+// one), the list of generated tokens and the step's result, which feeds it to the
+// next step.  -1, no token left, is kept in the list and fed as 0.
+static __global__ void commit_token_kernel(const int32_t* chosen, int32_t* history, int32_t* length,
+                                           int32_t* generated, StepResult* res) {
+  if (threadIdx.x != 0) return;
+  const int32_t t = *chosen;
+  history[*length] = t;
+  *length += 1;
+  *generated = t;
+  res->argmax_token = t < 0 ? 0u : (uint32_t)t;
+}
+
+void Engine::generate_processed(const uint32_t* prompt, size_t n_prompt, size_t n_gen, float repetition,
+                                float frequency, float presence, const int32_t* bias_ids,
+                                const float* bias_values, size_t n_bias, const uint32_t* mask,
+                                uint32_t* out_tokens) {
+  if (n_prompt == 0) throw std::runtime_error("empty prompt");
+  if (n_prompt + n_gen > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
+  if (tp_world_ > 1) throw std::runtime_error("generate_processed runs on one GPU");
+  if (!(repetition > 0.f) || !std::isfinite(repetition) || !std::isfinite(frequency) || !std::isfinite(presence))
+    throw std::runtime_error("penalties must be finite and repetition above 0");
+  if (n_bias > 65535) throw std::runtime_error("at most 65535 biases");
+  forward(prompt, n_prompt, 0);
+  if (n_gen == 0) return;
+  kv_ensure(n_prompt + n_gen);
+
+  // one buffer: history, generated tokens, {length, prompt length, chosen token},
+  // penalties, bias ids and values, mask words
+  const size_t V = arch_->V, words = (V + 31) / 32, hist = n_prompt + n_gen;
+  const size_t n32 = hist + n_gen + 3 + 3 + 2 * n_bias + (mask ? words : 0);
+  std::vector<uint32_t> host(n32, 0u);
+  uint32_t* at = host.data();
+  for (size_t i = 0; i < n_prompt; i++) at[i] = prompt[i];
+  uint32_t* state = at + hist + n_gen;
+  state[0] = state[1] = (uint32_t)n_prompt;
+  memcpy(state + 3, &repetition, 4);
+  memcpy(state + 4, &frequency, 4);
+  memcpy(state + 5, &presence, 4);
+  if (n_bias) {
+    memcpy(state + 6, bias_ids, n_bias * 4);
+    memcpy(state + 6 + n_bias, bias_values, n_bias * 4);
+  }
+  if (mask) memcpy(state + 6 + 2 * n_bias, mask, words * 4);
+  struct Buffer {
+    uint32_t* p = nullptr;
+    ~Buffer() {
+      if (p) cudaFree(p);
+    }
+  } buf;
+  CK(cudaMalloc(&buf.p, n32 * 4));
+  CK(cudaMemcpyAsync(buf.p, host.data(), n32 * 4, cudaMemcpyHostToDevice, stream_));
+  int32_t* const d_hist = reinterpret_cast<int32_t*>(buf.p);
+  int32_t* const d_out = d_hist + hist;
+  int32_t* const d_len = d_out + n_gen;
+  const float* const d_pen = reinterpret_cast<const float*>(d_len + 3);
+  const int32_t* const d_ids = d_len + 6;
+  const float* const d_vals = reinterpret_cast<const float*>(d_ids + n_bias);
+  const uint32_t* const d_mask = mask ? buf.p + hist + n_gen + 6 + 2 * n_bias : nullptr;
+
+  const int32_t one = 1, zero = 0;
+  CK(cudaMemcpyAsync(&d_st_->feed_argmax, &one, 4, cudaMemcpyHostToDevice, stream_));
+  CK(cudaMemcpyAsync(&d_st_->n_gen, &zero, 4, cudaMemcpyHostToDevice, stream_));
+  for (size_t i = 0; i < n_gen; i++) {
+    if (i > 0) run_steps(1);
+    const int rc = chpe_logits_process(
+        d_logits_, CHPE_F32, (int64_t)V, 1, (uint32_t)V, d_hist, (int64_t)hist, (uint32_t)hist, d_len + 1, d_len,
+        repetition != 1.f ? d_pen : nullptr, frequency != 0.f ? d_pen + 1 : nullptr,
+        presence != 0.f ? d_pen + 2 : nullptr, n_bias ? d_ids : nullptr, n_bias ? d_vals : nullptr, 0,
+        (uint32_t)n_bias, d_mask, 0, nullptr, 0, d_len + 2, stream_);
+    if (rc != 0) throw std::runtime_error(chpe_last_error(nullptr));
+    commit_token_kernel<<<1, 32, 0, stream_>>>(d_len + 2, d_hist, d_len, d_out + i, d_res_);
+    CK(cudaGetLastError());
+  }
+  CK(cudaMemcpyAsync(out_tokens, d_out, n_gen * 4, cudaMemcpyDeviceToHost, stream_));
+  CK(cudaMemcpyAsync(&d_st_->feed_argmax, &zero, 4, cudaMemcpyHostToDevice, stream_));
+  sync_result();
+  pos_ = (uint32_t)(n_prompt + n_gen - 1);
+  for (size_t i = 0; i < n_gen; i++)
+    if (out_tokens[i] == 0xFFFFFFFFu)
+      throw std::runtime_error("no token is allowed at generated token " + std::to_string(i));
 }
 
 void Engine::verify(const uint32_t* toks, size_t m, uint32_t pos, float* logits_out, uint32_t* argmax_out) {

@@ -58,6 +58,14 @@ class Engine {
   // Greedy generation on the device: prompt (n_prompt) then n_gen steps
   // feeding each argmax back as the next token; out_tokens gets n_gen ids.
   void generate(const uint32_t* prompt, size_t n_prompt, size_t n_gen, uint32_t* out_tokens);
+  // generate() with the sampling rules of chpe_logits_process on every step's
+  // logits: penalties over the prompt and the tokens written so far, biases, and
+  // a mask (vocab bits, or null) that holds for every step.  Throws when a step
+  // is left without a token.
+  void generate_processed(const uint32_t* prompt, size_t n_prompt, size_t n_gen, float repetition,
+                          float frequency, float presence, const int32_t* bias_ids,
+                          const float* bias_values, size_t n_bias, const uint32_t* mask,
+                          uint32_t* out_tokens);
   // Batch-M verification: logits of m candidate tokens scored at positions
   // pos..pos+m-1, each seeing the KV entries of the ones before it (causal),
   // i.e. m forwardDecode steps; logits_out [m][vocab], argmax_out [m] (either

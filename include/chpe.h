@@ -181,6 +181,20 @@ const char *chpe_verify_batched_unavailable(void *ctx, int m);
 int chpe_generate(void *ctx, const uint32_t *prompt, size_t n_prompt, size_t n_gen,
                   uint32_t *out_tokens);
 
+/* chpe_generate with the rules of chpe_logits_process (below) on every step's
+ * logits before its token is chosen: the penalties over the prompt and the
+ * tokens written so far (repetition 1, frequency 0, presence 0: none), n_bias
+ * biases (host arrays; of several for one token the last counts), and a mask of
+ * ceil(vocab/32) host words that holds for every step (NULL: none).  With no
+ * rule it gives chpe_generate's tokens.  chpe_get_last_logits gives the last
+ * step's logits as the model gave them.  One GPU.  0 on success; -1 on error, among
+ * them penalties that are not finite, a repetition of 0 or less, and a step that
+ * is left without a token (out_tokens holds 0xFFFFFFFF there). */
+int chpe_generate_processed(void *ctx, const uint32_t *prompt, size_t n_prompt, size_t n_gen,
+                            float repetition, float frequency, float presence,
+                            const int32_t *bias_ids, const float *bias_values, size_t n_bias,
+                            const uint32_t *mask, uint32_t *out_tokens);
+
 /* Speculative greedy generation (an extension; the reference has no
  * speculative decoding): like chpe_generate, but after the prompt each round
  * drafts up to draft_len tokens by prompt lookup (the tokens that followed
