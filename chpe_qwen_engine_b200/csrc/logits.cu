@@ -10,8 +10,8 @@
 // argmax: the lowest index of the largest x; NaN never wins; -1 when nothing
 // is above -inf.
 //
-// Bound by memory: the logits in, the f32 logits out.  A cluster of 8 CTAs takes
-// one row; tiles of 128 tokens (a warp's four per lane) go to the CTAs in turn, so
+// Bound by memory: the logits in, the f32 logits out.  A cluster of 8 or 16 CTAs
+// takes one row; tiles of 128 tokens (a warp's four per lane) go to the CTAs in turn, so
 // that the frequent tokens, which have low ids, are spread over them.  Three steps:
 //   1. table: the CTA's tokens of the history are counted in shared memory (one
 //      entry per token: the top bit seen in the prompt, the rest the count after it;
@@ -41,8 +41,8 @@
 
 namespace {
 
-constexpr uint32_t kCluster = 8;
-constexpr int kMaxThreads = 1024;
+constexpr uint32_t kMaxCluster = 16;
+constexpr int kMaxThreads = 512;
 constexpr uint32_t kTile = 128;
 constexpr uint32_t kChunk = 28672;  // most tokens of a CTA counted at a time (up to 8 bytes each)
 constexpr int kAhead = 4;  // steps of the stream, and
@@ -51,6 +51,7 @@ constexpr int kIds = 4;    // ids of the history, whose loads a thread has in fl
 struct LogitsLaunch {
   const void* logits;
   int64_t stride;
+  uint32_t lg;  // log2 of the CTAs of a row
   uint32_t vocab, chunk;  // chunk: tokens a CTA takes at a time (a multiple of kTile)
   const int32_t* history;
   int64_t history_stride;
@@ -134,8 +135,7 @@ struct Raw4 {
 // E: bytes of a table entry (0: neither history nor biases).  VEC: rows and the
 // output start at multiples of four tokens' bytes.
 template <typename T, int E, bool BIAS, bool VEC>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
-    logits_kernel(const __grid_constant__ LogitsLaunch P) {
+__global__ void __launch_bounds__(kMaxThreads) logits_kernel(const __grid_constant__ LogitsLaunch P) {
   constexpr uint32_t kSeen = E == 2 ? 0x8000u : 0x80000000u, kBiased = kSeen >> 1;
   extern __shared__ __align__(16) unsigned char smem[];
   uint32_t* const table = reinterpret_cast<uint32_t*>(smem);  // [chunk] entries of E bytes
@@ -143,23 +143,23 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
   uint16_t* const list = reinterpret_cast<uint16_t*>(which + (BIAS ? P.slots / 2 : 0));  // tokens with an entry
   __shared__ uint32_t listed;
   __shared__ unsigned long long best_of[kMaxThreads / 32];
-  __shared__ unsigned long long cta_best[kCluster];
+  __shared__ unsigned long long cta_best[kMaxCluster];
   const uint32_t tid = threadIdx.x, rank = cluster_rank(), nt = blockDim.x;
   if (P.argmax) cluster_arrive();  // every CTA of the cluster has started: waited for at the end
-  const int64_t row = blockIdx.x / kCluster;
+  const int64_t row = blockIdx.x >> P.lg;
   const T* const x_row = static_cast<const T*>(P.logits) + row * P.stride;
   float* const out = P.out ? P.out + row * P.out_stride : nullptr;
   const uint32_t* const mask = P.mask ? P.mask + row * P.mask_stride : nullptr;
   // the CTA's i-th token, and the place of token v among them (0xFFFFFFFF: another CTA's, or none)
-  auto token = [&](uint32_t i) { return ((i / kTile) * kCluster + rank) * kTile + i % kTile; };
+  auto token = [&](uint32_t i) { return (((i / kTile) << P.lg) + rank) * kTile + i % kTile; };
   auto place = [&](uint32_t v) {
     const uint32_t tile = v / kTile;
-    return v < P.vocab && tile % kCluster == rank ? tile / kCluster * kTile + v % kTile : 0xFFFFFFFFu;
+    return v < P.vocab && (tile & ((1u << P.lg) - 1u)) == rank ? (tile >> P.lg) * kTile + v % kTile : 0xFFFFFFFFu;
   };
   // where the search for a biased token's entry begins
   auto slot_of = [&](uint32_t o) { return P.slots == P.chunk ? o : (o * 0x9E3779B1u) >> P.slot_shift; };
   const uint32_t tiles = (P.vocab + kTile - 1) / kTile;
-  const uint32_t mine = rank < tiles ? ((tiles - rank - 1) / kCluster + 1) * kTile : 0;  // the last may be cut
+  const uint32_t mine = rank < tiles ? (((tiles - rank - 1) >> P.lg) + 1) * kTile : 0;  // the last may be cut
 
   float best = -INFINITY;
   uint32_t best_v = 0;
@@ -169,6 +169,26 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
       best_v = v;
     }
   };
+  // what the later steps wait for is asked for first: the row's lengths and penalties,
+  // the first ids of its history and its first bias
+  uint32_t total = 0, prompt = 0, first_id[kIds], first_bias = 0xFFFFFFFFu;
+  float rep = 1.f, freq = 0.f, pres = 0.f;
+  const int32_t* const hist = P.history ? P.history + row * P.history_stride : nullptr;
+  const int32_t* const ids = BIAS ? P.bias_ids + row * P.bias_stride : nullptr;
+  if constexpr (E != 0) {
+    if (hist) {
+#pragma unroll
+      for (int j = 0; j < kIds; j++) first_id[j] = tid + j * nt < P.history_len ? (uint32_t)hist[tid + j * nt] : 0xFFFFFFFFu;
+      const int m = P.total_lens ? P.total_lens[row] : (int)P.history_len;
+      total = m < 0 ? 0u : min((uint32_t)m, P.history_len);
+      const int p = P.prompt_lens ? P.prompt_lens[row] : 0;
+      prompt = p < 0 ? 0u : (uint32_t)p;
+      if (P.repetition) rep = P.repetition[row];
+      if (P.frequency) freq = P.frequency[row];
+      if (P.presence) pres = P.presence[row];
+    }
+    if (BIAS && tid < P.max_bias) first_bias = (uint32_t)ids[tid];
+  }
   for (uint32_t c0 = 0; c0 < mine; c0 += P.chunk) {
     const uint32_t n = min(P.chunk, mine - c0);
     Raw4<T> raw[kAhead];
@@ -184,19 +204,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
 #pragma unroll
       for (int u = 0; u < kAhead; u++) fetch(u, 4 * (tid + u * nt));
 
-    uint32_t total = 0, prompt = 0;
-    const int32_t* const hist = P.history ? P.history + row * P.history_stride : nullptr;
-    const int32_t* const ids = BIAS ? P.bias_ids + row * P.bias_stride : nullptr;
     if constexpr (E != 0) {
       if (c0) __syncthreads();  // the previous chunk's table is read
       const uint32_t words = P.chunk / 4 * E + (BIAS ? P.slots / 2 : 0);
       for (uint32_t i = tid; i < words / 4; i += nt) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
-      if (hist) {
-        const int m = P.total_lens ? P.total_lens[row] : (int)P.history_len;
-        total = m < 0 ? 0u : min((uint32_t)m, P.history_len);
-        const int p = P.prompt_lens ? P.prompt_lens[row] : 0;
-        prompt = p < 0 ? 0u : (uint32_t)p;
-      }
       if (tid == 0) listed = 0;
       __syncthreads();
       auto flag = [&](uint32_t o, uint32_t f) {
@@ -207,7 +218,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
       for (uint32_t i0 = tid; i0 < total; i0 += kIds * nt) {
         uint32_t id[kIds];
 #pragma unroll
-        for (int j = 0; j < kIds; j++) id[j] = i0 + j * nt < total ? (uint32_t)hist[i0 + j * nt] : 0xFFFFFFFFu;
+        for (int j = 0; j < kIds; j++)
+          id[j] = i0 + j * nt >= total ? 0xFFFFFFFFu : i0 == tid ? first_id[j] : (uint32_t)hist[i0 + j * nt];
 #pragma unroll
         for (int j = 0; j < kIds; j++) {
           const uint32_t o = place(id[j]) - c0;
@@ -218,7 +230,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
       }
       if constexpr (BIAS) {
         for (uint32_t i = tid; i < P.max_bias; i += nt) {
-          const uint32_t id = (uint32_t)ids[i], o = place(id) - c0;
+          const uint32_t id = i == tid ? first_bias : (uint32_t)ids[i], o = place(id) - c0;
           if (o >= n) continue;
           flag(o, kBiased);
           uint32_t k = slot_of(o);  // at most half of the slots are taken: the search ends before it is back
@@ -306,8 +318,6 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
     }
 
     if constexpr (E != 0) {
-      const float rep = P.repetition ? P.repetition[row] : 1.f;
-      const float freq = P.frequency ? P.frequency[row] : 0.f, pres = P.presence ? P.presence[row] : 0.f;
       __syncthreads();  // step 3 writes over what other threads wrote
       for (uint32_t k = tid; k < listed; k += nt) {
         const uint32_t o = list[k], v = token(c0 + o);
@@ -356,7 +366,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kMaxThreads)
   cluster_arrive();  // rank 0 alone stays for the others' keys
   if (rank != 0) return;
   cluster_wait();
-  key = tid < kCluster ? *reinterpret_cast<volatile unsigned long long*>(&cta_best[tid]) : 0ull;
+  key = tid < 1u << P.lg ? *reinterpret_cast<volatile unsigned long long*>(&cta_best[tid]) : 0ull;
   warp_key();
   if (tid == 0) P.argmax[row] = key ? (int32_t)(0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFull)) : -1;
 }
@@ -373,24 +383,29 @@ cudaError_t launch(LogitsLaunch P, uint32_t batch, int device, cudaStream_t s) {
   uint64_t entries = (P.history ? P.history_len : 0u) + (uint64_t)(BIAS ? P.max_bias : 0u);
   if (entries > P.chunk) entries = P.chunk;
   const int bytes = E ? (int)(P.chunk * E + (BIAS ? 2 * P.slots : 0) + 2 * entries) : 0;
-  if (bytes > 40 * 1024) {
-    static int set[64] = {};  // per device: done once
-    const int dev = device >= 0 && device < 64 ? device : -1;
-    if (dev < 0 || !__atomic_load_n(&set[dev], __ATOMIC_RELAXED)) {
-      const cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, E, BIAS, VEC>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)(kChunk * (E + (BIAS ? 2 : 0) + 2)));
-      if (e != cudaSuccess) return e;
-      if (dev >= 0) __atomic_store_n(&set[dev], 1, __ATOMIC_RELAXED);
-    }
+  auto kernel = logits_kernel<T, E, BIAS, VEC>;
+  static int set[64] = {};  // per device: done once
+  const int dev = device >= 0 && device < 64 ? device : -1;
+  if (dev < 0 || !__atomic_load_n(&set[dev], __ATOMIC_RELAXED)) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)(kChunk * (E + (BIAS ? 2 : 0) + 2)));
+    if (e != cudaSuccess) return e;
+    if (dev >= 0) __atomic_store_n(&set[dev], 1, __ATOMIC_RELAXED);
   }
-  // Few CTAs are waited for by their loads: many threads each (one row of 151936 with a
-  // history: 7.9 us with 1024, 9.1 with 256; 24 rows: 18.1 with 1024, 12.6 with 512,
-  // 14.5 with 256).  Many CTAs overlap one another's phases best when small (64
-  // rows: 47, 26, 21.9 us; 256 rows: 129, 85, 69 us).
-  const int threads = batch * kCluster <= 80 ? 1024 : batch * kCluster <= 192 ? 512 : 256;
-  logits_kernel<T, E, BIAS, VEC><<<batch * kCluster, threads, bytes, s>>>(P);
-  return cudaGetLastError();
+  const uint32_t ctas = batch << P.lg;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(batch <= 32 ? 512 : 256);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {1u << P.lg, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P);
 }
 
 template <typename T, bool VEC>
@@ -458,7 +473,12 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
 
   LogitsLaunch P{};
   P.logits = logits, P.stride = logits_stride, P.vocab = vocab;
-  const uint32_t tiles = (vocab + kTile - 1) / kTile, each = (tiles + kCluster - 1) / kCluster;
+  // Few rows are waited for by their loads: 16 CTAs of 512 threads each.  Many
+  // overlap one another's phases best when the CTAs are small.  All rules, rows of 152064,
+  // us with 16 x 512 / 8 x 512 / 8 x 256: 5 rows 7.4 / 9.6 / 12.0, 14 rows 9.8 / 9.9 /
+  // 12.4, 18 rows 15.2 / 12.5 / 14.1, 32 rows 25 / 14.1 / 16.6, 48 rows 34 / 24.5 / 19.3.
+  P.lg = batch <= 14 ? 4 : 3;
+  const uint32_t tiles = (vocab + kTile - 1) / kTile, each = (tiles + (1u << P.lg) - 1) >> P.lg;
   P.chunk = each < kChunk / kTile ? each * kTile : kChunk;
   if (history_len) P.history = history, P.history_stride = history_stride, P.history_len = history_len;
   P.prompt_lens = prompt_lens, P.total_lens = total_lens;
@@ -468,7 +488,7 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
   P.out = out, P.out_stride = out_stride, P.argmax = argmax;
   const bool vec = reinterpret_cast<uintptr_t>(logits) % (4 * es) == 0 && (batch == 1 || logits_stride % 4 == 0) &&
                    (!out || (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (batch == 1 || out_stride % 4 == 0)));
-  chpe::DeviceScope scope(c.device);
+  chpe::DeviceScope scope(c.launch_device());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == CHPE_F32) e = launch_type<float>(P, batch, vec, c.device, s);

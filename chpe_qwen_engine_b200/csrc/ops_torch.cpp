@@ -27,6 +27,9 @@ using at::Tensor;
 struct Unfit : std::runtime_error {  // becomes ValueError
   using std::runtime_error::runtime_error;
 };
+struct Misuse : std::runtime_error {  // becomes TypeError
+  using std::runtime_error::runtime_error;
+};
 void want(bool ok, const char* what) {
   if (!ok) throw Unfit(what);
 }
@@ -59,7 +62,7 @@ struct Args {
 
   // names[0..positional) may be given by position, all of them by name
   void parse(PyObject* const* names, int positional, PyObject* const* args, Py_ssize_t n, PyObject* kw, const char* fn) {
-    if (n > positional) unfit(std::string(fn) + " takes " + std::to_string(positional) + " arguments by position");
+    if (n > positional) throw Misuse(std::string(fn) + " takes " + std::to_string(positional) + " arguments by position");
     for (Py_ssize_t i = 0; i < n; i++) at[i] = args[i];
     const Py_ssize_t k = kw ? PyTuple_GET_SIZE(kw) : 0;
     for (Py_ssize_t j = 0; j < k; j++) {
@@ -70,7 +73,8 @@ struct Args {
         for (i = 0; i < N && PyUnicode_Compare(names[i], key) != 0;) i++;
       if (i == N || (i < n)) {
         const char* s = PyUnicode_AsUTF8(key);
-        unfit(std::string(fn) + (i == N ? ": unknown argument " : ": given twice: ") + (s ? s : "?"));
+        if (!s) PyErr_Clear();
+        throw Misuse(std::string(fn) + (i == N ? ": unknown argument " : ": given twice: ") + (s ? s : "?"));
       }
       at[i] = args[n + j];
     }
@@ -79,10 +83,10 @@ struct Args {
   }
   const Tensor* tensor(int i, const char* name, bool needed = false) const {
     if (!at[i]) {
-      if (needed) unfit(std::string(name) + " is missing");
+      if (needed) throw Misuse(std::string(name) + " is missing");
       return nullptr;
     }
-    if (!THPVariable_Check(at[i])) unfit(std::string(name) + " must be a tensor");
+    if (!THPVariable_Check(at[i])) throw Misuse(std::string(name) + " must be a tensor");
     return &THPVariable_Unpack(at[i]);
   }
   double number(int i, const char* name, double def) const {
@@ -90,7 +94,7 @@ struct Args {
     const double v = PyFloat_AsDouble(at[i]);
     if (v == -1.0 && PyErr_Occurred()) {
       PyErr_Clear();
-      unfit(std::string(name) + " must be a number");
+      throw Misuse(std::string(name) + " must be a number");
     }
     return v;
   }
@@ -161,6 +165,8 @@ PyObject* guarded(F f) {
     return f();
   } catch (const Unfit& e) {
     PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const Misuse& e) {
+    PyErr_SetString(PyExc_TypeError, e.what());
   } catch (const Refused&) {
     PyObject* pkg = PyImport_ImportModule("chpe_qwen_engine_b200");
     PyObject* type = pkg ? PyObject_GetAttrString(pkg, "ChpeError") : nullptr;
@@ -332,7 +338,8 @@ PyObject* logits_process(PyObject*, PyObject* const* args, Py_ssize_t n, PyObjec
     want(x.dim() == 2, "logits must be [batch, vocab]");
     const int64_t B = x.size(0), V = x.size(1);
     const int64_t xs = rows_of(x, "logits", x.scalar_type(), dev, B, V);
-    const bool full = !a.at[WANT] || PyObject_IsTrue(a.at[WANT]) == 1;
+    const int full = a.at[WANT] ? PyObject_IsTrue(a.at[WANT]) : 1;
+    if (full < 0) return nullptr;
     Tensor made, best;
     const Tensor *out = a.tensor(OUT, "out"), *am = a.tensor(ARGMAX, "argmax");
     if (!out && full) out = &(made = make({B, V}, at::kFloat, dev));

@@ -348,7 +348,7 @@ extern "C" int chpe_qk_norm_rope(const void* q, const void* k, const void* v, in
   P.H = (int32_t)num_heads, P.KV = (int32_t)num_kv_heads;
   P.k_cache = k_cache, P.v_cache = v_cache, P.slots = k_cache ? slots : nullptr;
   P.cache_rows = (int64_t)cache_rows;
-  chpe::DeviceScope scope(c.device);
+  chpe::DeviceScope scope(c.launch_device());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool half = !k_cache ? dtype != CHPE_BF16 : cache_dtype == CHPE_F16;
   cudaError_t e;

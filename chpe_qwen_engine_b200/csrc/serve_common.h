@@ -68,6 +68,11 @@ struct ServeCall {
   void ptr_or_null(const void* p, const char* what, uintptr_t align) {
     if (p) ptr(p, what, align);
   }
+  // The device to launch on: that of the buffers, or the current one for managed memory.
+  int launch_device() {
+    if (device < 0 && cudaGetDevice(&device) != cudaSuccess) device = 0;
+    return device;
+  }
   // Ends the call: keeps the message for chpe_last_error(NULL).
   int done() const {
     try {

@@ -270,7 +270,9 @@ uint32_t chpe_get_position(void *ctx);
  * 1/world of the weights. */
 uint64_t chpe_device_archive_bytes(void *ctx);
 /* Last error message of ctx, or, when ctx is NULL, of the calling thread's
- * last failed init or chpe_attention_decode_noalloc call; "" when none. */
+ * last failed init, or its last call of an entry point without a context
+ * (chpe_attention_decode_noalloc, chpe_convert_archive, the operators of a
+ * batched decode step); "" when none. */
 const char *chpe_last_error(void *ctx);
 
 /* Paged KV cache (an extension; the reference keeps one contiguous f32

@@ -96,7 +96,8 @@ def logits(x, history=None, prompt=None, total=None, rep=None, freq=None, pres=N
         if ids is not None:
             last = {int(i): kind(v) for i, v in zip(ids[b], vals[b]) if 0 <= i < V}
             for i, v in last.items():
-                x[b, i] = x[b, i] + v
+                with np.errstate(all="ignore"):
+                    x[b, i] = x[b, i] + v
         if mask is not None:
             w = mask[b].astype(np.int64) & 0xFFFFFFFF
             t = np.arange(V)

@@ -155,3 +155,19 @@ def test_definition_of_the_rules():
     y, a = logits(x, mask=m)
     assert np.array_equal(np.isneginf(y[0]), [False, False, True, True, False, True]) and a[0] == 0
     assert logits(x, mask=np.zeros((1, 1), np.int64))[1][0] == -1
+
+
+def test_torch_layer_arguments():
+    torch = pytest.importorskip("torch")
+    from chpe_qwen_engine_b200 import ops
+    x = torch.zeros(2, 8)
+    with pytest.raises(TypeError, match="unknown argument penalty"):
+        ops.logits_process(x, penalty=1)
+    with pytest.raises(TypeError, match="by position"):
+        ops.logits_process(x, None)
+    with pytest.raises(TypeError, match="given twice"):
+        ops.qk_norm_rope(x, x, q=x)
+    with pytest.raises(TypeError, match="logits is missing"):
+        ops.logits_process()
+    with pytest.raises(TypeError, match="must be a tensor"):
+        ops.logits_process(3)
