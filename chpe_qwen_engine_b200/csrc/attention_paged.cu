@@ -230,6 +230,7 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
   const int cta = blockIdx.x, n_cta = gridDim.x;
   const int hw = warp & (P.HW - 1), sub = warp >> (31 - __clz(P.HW)), subs = 1 << (P.tile_shift - 4);
 
+  pdl_wait();
   // ---- this CTA's stretch of the line of tiles
   const int per = (P.B + THREADS - 1) / THREADS;
   const int b_lo = min(tid * per, P.B), b_hi = min(b_lo + per, P.B);
@@ -595,6 +596,7 @@ __global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant_
   __shared__ float sv[kRows][DB];
   __shared__ float red[2][JW];
   pdl_wait();
+  pdl_launch_dependents();
   const int4 cut = P.desc[blockIdx.x];
   const int n = cut.z;  // at most one record per CTA
   if (n == 0) return;
@@ -696,30 +698,20 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   P.by_seq = (int64_t)P.B * P.groups <= grid;
   P.desc = static_cast<int4*>(workspace);
   P.part = reinterpret_cast<float*>(P.desc + C::kMaxCtas);
-  paged_kernel<T, TQ, D><<<grid, 32 * C::kWarps, C::kRing + (subs - 1) * P.HW * C::kSums * sizeof(float), s>>>(P);
-  const cudaError_t e = cudaGetLastError();
+  chpe::ServeLaunch main(dim3(grid), 32 * C::kWarps, C::kRing + (subs - 1) * P.HW * C::kSums * sizeof(float), s);
+  const cudaError_t e = cudaLaunchKernelEx(&main.cfg, paged_kernel<T, TQ, D>, P);
   if (e != cudaSuccess) return e;
-  // started while the kernel above ends; it waits for it before it reads anything
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.stream = s;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
   const int cuts = P.by_seq ? P.B * P.groups : grid;
   // The records that a group may be cut into: many are joined by many threads (one
   // sequence of 8192 on 64/8 heads: 16.0 us, with two warps per query head 20.2),
   // few by two warps (16 sequences of 150 on 16/2 heads: 8.2 us, with 16 warps 11.0).
   const int64_t records = (P.cap >> P.tile_shift) < grid / cuts + 2 ? (P.cap >> P.tile_shift) : grid / cuts + 2;
   if (records > 16) {
-    cfg.gridDim = dim3(cuts, P.HW * kHeads * (D / 64));
-    cfg.blockDim = dim3(32 * 16);
-    return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, 64, 16>, P);
+    chpe::ServeLaunch join(dim3(cuts, P.HW * kHeads * (D / 64)), 32 * 16, 0, s);
+    return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, 64, 16>, P);
   }
-  cfg.gridDim = dim3(cuts, P.HW * kHeads);
-  cfg.blockDim = dim3(32 * 2);
-  return cudaLaunchKernelEx(&cfg, combine_kernel<TQ, D, D, 2>, P);
+  chpe::ServeLaunch join(dim3(cuts, P.HW * kHeads), 32 * 2, 0, s);
+  return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, D, 2>, P);
 }
 
 template <typename T, typename TQ>

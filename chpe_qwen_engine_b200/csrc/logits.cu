@@ -145,6 +145,8 @@ __global__ void __launch_bounds__(kMaxThreads) logits_kernel(const __grid_consta
   __shared__ unsigned long long best_of[kMaxThreads / 32];
   __shared__ unsigned long long cta_best[kMaxCluster];
   const uint32_t tid = threadIdx.x, rank = cluster_rank(), nt = blockDim.x;
+  pdl_wait();
+  pdl_launch_dependents();
   if (P.argmax) cluster_arrive();  // every CTA of the cluster has started: waited for at the end
   const int64_t row = blockIdx.x >> P.lg;
   const T* const x_row = static_cast<const T*>(P.logits) + row * P.stride;
@@ -394,18 +396,8 @@ cudaError_t launch(LogitsLaunch P, uint32_t batch, int device, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     if (dev >= 0) __atomic_store_n(&set[dev], 1, __ATOMIC_RELAXED);
   }
-  const uint32_t ctas = batch << P.lg;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(batch <= 32 ? 512 : 256);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {1u << P.lg, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, P);
+  chpe::ServeLaunch L(dim3(batch << P.lg), batch <= 32 ? 512 : 256, bytes, s, 1u << P.lg);
+  return cudaLaunchKernelEx(&L.cfg, kernel, P);
 }
 
 template <typename T, bool VEC>

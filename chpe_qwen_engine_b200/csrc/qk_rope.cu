@@ -142,6 +142,8 @@ template <typename TA, typename TC, int D, int U>
 __global__ void __launch_bounds__(32 * kWarps) qk_rope_kernel(const __grid_constant__ QkLaunch P) {
   constexpr int LPH = D / 16, HPG = 32 / LPH;  // lanes per head, heads per group
   __shared__ float2 cs[kWarps][kMaxHalf];
+  pdl_wait();
+  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t id = blockIdx.x * kWarps + warp;
   if (id >= P.warps) return;
@@ -265,8 +267,8 @@ cudaError_t launch(QkLaunch& P, uint32_t tokens, cudaStream_t s) {
   // (more warps than 32 bits can count: whole tokens)
   if ((uint64_t)tokens * P.runs > 0xffffff00u) P.runs = 1;
   P.warps = tokens * (uint32_t)P.runs;
-  qk_rope_kernel<TA, TC, D, U><<<(P.warps + kWarps - 1) / kWarps, 32 * kWarps, 0, s>>>(P);
-  return cudaGetLastError();
+  chpe::ServeLaunch L(dim3((P.warps + kWarps - 1) / kWarps), 32 * kWarps, 0, s);
+  return cudaLaunchKernelEx(&L.cfg, qk_rope_kernel<TA, TC, D, U>, P);
 }
 
 template <typename TA, typename TC>

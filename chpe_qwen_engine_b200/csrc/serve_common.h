@@ -101,6 +101,30 @@ class DeviceScope {
   bool changed_ = false;
 };
 
+// Launch attributes: the kernel may be started while the one before it in the
+// stream ends (programmatic dependent launch); each kernel here waits for that one before it
+// reads or writes anything.
+struct ServeLaunch {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[2];
+  ServeLaunch(dim3 grid, unsigned threads, size_t smem, cudaStream_t s, unsigned cluster = 1) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = at;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster > 1) {
+      at[1].id = cudaLaunchAttributeClusterDimension;
+      at[1].val.clusterDim.x = cluster;
+      at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+      cfg.numAttrs = 2;
+    }
+  }
+};
+
 inline size_t dtype_size(int t) { return t == CHPE_F32 ? 4 : (t == CHPE_F16 || t == CHPE_BF16) ? 2 : 0; }
 
 }  // namespace chpe
