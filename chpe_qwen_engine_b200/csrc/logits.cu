@@ -27,7 +27,8 @@
 // The CTAs join their best tokens through distributed shared memory: no
 // workspace, no second launch.  Without history and biases only step 2 is left.
 // 256 rows of 151936 BF16 logits: 55 us as they are (4.2 TB/s; a plain cast of
-// them to f32 by the library takes 103), 69 with histories of up to 8191.
+// them to f32 by the library takes 103), 69 with histories of up to 8191.  In
+// place, only what changes is written.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -67,6 +68,7 @@ struct LogitsLaunch {
   int64_t mask_stride;
   float* out;
   int64_t out_stride;
+  int32_t in_place;  // out is the logits: what the mask leaves as it is need not be written
   int32_t* argmax;
 };
 
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kMaxThreads) logits_kernel(const __grid_consta
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] = allowed >> j & 1u ? x[j] : -INFINITY;
           }
-          if (out) *reinterpret_cast<float4*>(out + v) = make_float4(x[0], x[1], x[2], x[3]);
+          if (out && !(P.in_place && (!mask || (allowed & 0xFu) == 0xFu))) *reinterpret_cast<float4*>(out + v) = make_float4(x[0], x[1], x[2], x[3]);
           if constexpr (E != 0) {  // tokens that step 3 comes back to
             const uint32_t later = entries4(i);
             if (later) {
@@ -311,8 +313,9 @@ __global__ void __launch_bounds__(kMaxThreads) logits_kernel(const __grid_consta
       const uint32_t v = token(c0 + i);
       if (v >= P.vocab || (VEC && v < (P.vocab & ~3u))) continue;
       float x = to_float<T>(x_row[v]);
-      if (mask && !(mask[v >> 5] >> (v & 31u) & 1u)) x = -INFINITY;
-      if (out) out[v] = x;
+      const bool banned = mask && !(mask[v >> 5] >> (v & 31u) & 1u);
+      if (banned) x = -INFINITY;
+      if (out && (banned || !P.in_place)) out[v] = x;
       bool open = true;
       if constexpr (E != 0) open = !(entries4(i & ~3u) >> (i & 3u) & 1u);
       if (open) offer(x, v);
@@ -478,6 +481,7 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
   if (max_bias) P.bias_ids = bias_ids, P.bias_values = bias_values, P.bias_stride = bias_stride, P.max_bias = max_bias;
   P.mask = mask, P.mask_stride = mask_stride;
   P.out = out, P.out_stride = out_stride, P.argmax = argmax;
+  P.in_place = dtype == CHPE_F32 && out == logits && (batch == 1 || out_stride == logits_stride);
   const bool vec = reinterpret_cast<uintptr_t>(logits) % (4 * es) == 0 && (batch == 1 || logits_stride % 4 == 0) &&
                    (!out || (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (batch == 1 || out_stride % 4 == 0)));
   chpe::DeviceScope scope(c.launch_device());
