@@ -29,8 +29,8 @@
 // waits for no other warp; only warps that share a head meet, at the end of a part.
 //
 // Measured (device time): 131071 positions of one sequence on 64/8 heads of 128: 92 us,
-// 90 % of the copy rate; 64 sequences of up to 8192 there: 124 us, 90 %; 37 of up
-// to 4093 on 16/4 heads of 256: 52 us, 62 %; one of 77 on 16/2 heads: 7.6 us.
+// 91 % of the copy rate; 64 sequences of up to 8192 there: 125 us, 90 %; 37 of up
+// to 4093 on 16/4 heads of 256: 45 us, 72 %; one of 77 on 16/2 heads: 7.9 us.
 // What is left: SMs get bandwidth unevenly, so that CTAs with equal shares end
 // 10 % before and after the mean, and the records' join, 3 us behind a gap of 2.
 // Handing a fifth of the line out to whoever is done evened the ends out but cost as

@@ -343,7 +343,7 @@ int chpe_attention_decode_noalloc(const float *q, const float *k, const float *v
  * streams may overlap (attention: with a workspace each).
  * Return value: 0; -1 for an argument they refuse (NULL, misaligned or host
  * pointers, sizes and types outside the limits), -2 for too small a workspace,
- * -3 for a CUDA error at the launch; nothing is launched then and
+ * -3 for a CUDA error at the launch (the outputs are undefined then);
  * chpe_last_error(NULL) says why. */
 #define CHPE_F32 0
 #define CHPE_F16 1
