@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
 }
 
 // Joins the records of a cut group: blockIdx.x the desc entry, blockIdx.y the
-// query head within the group and the DB of its D values.  The records' weights
+// query head within the group and the DB of its D values, JW warps.  The records' weights
 // are worked out once, side by side; 4 * DB bytes of a record take DB/4 lanes, and every
 // lane has kBatch records' loads in flight.
 template <typename TQ, int D, int DB, int JW>
@@ -669,6 +669,67 @@ __global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant_
     P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
 }
 
+// The same where a group is cut into a few records only: a warp per query head, 8
+// heads to a CTA, no barrier.  blockIdx.x the desc entry, blockIdx.y the head's warp of
+// the main kernel.
+template <typename TQ, int D>
+__global__ void __launch_bounds__(32 * kHeads) combine_few_kernel(const __grid_constant__ PagedLaunch P) {
+  using C = Cfg<D>;
+  constexpr int PER = D / 64, kBatch = D == 256 ? 4 : 8;  // pairs of a lane, records in flight
+  pdl_wait();
+  pdl_launch_dependents();
+  const int4 cut = P.desc[blockIdx.x];
+  const int n = cut.z;
+  if (n == 0) return;
+  const int hw = blockIdx.y, h = threadIdx.x >> 5, lane = threadIdx.x & 31, vh = cut.y * P.HW + hw;
+  const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * kHeads + h;
+  if (head >= (kvh + 1) * P.G) return;
+  auto rec = [&](int i) { return P.part + (((size_t)2 * (cut.w + i) + (i == 0 ? 1 : 0)) * P.HW + hw) * C::kRec; };
+  float2 x[kBatch][PER];
+  auto fetch = [&](int j, int i) {
+#pragma unroll
+    for (int e = 0; e < PER; e++)
+      x[j][e] = i < n ? *reinterpret_cast<const float2*>(rec(i) + h * D + 64 * e + 2 * lane) : make_float2(0.f, 0.f);
+  };
+#pragma unroll
+  for (int j = 0; j < kBatch; j++) fetch(j, j);
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, rec(i)[kHeads * D + 2 * h]);
+  M = warp_max(M);
+  float2 v[PER];
+#pragma unroll
+  for (int e = 0; e < PER; e++) v[e] = make_float2(0.f, 0.f);
+  float L = 0.f;
+  for (int c = 0; c < n; c += 32) {  // 32 records' weights at a time
+    float w = 0.f;
+    if (c + lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(rec(c + lane) + kHeads * D + 2 * h);
+      w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+      L = fmaf(ml.y, w, L);  // a NaN sum stays
+    }
+    const int end = min(32, n - c);
+    for (int i0 = 0; i0 < end; i0 += kBatch) {
+#pragma unroll
+      for (int j = 0; j < kBatch; j++) {
+        const float wi = __shfl_sync(0xffffffffu, w, (i0 + j) & 31);  // 0 behind the last
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+          v[e].x = fmaf(x[j][e].x, wi, v[e].x);
+          v[e].y = fmaf(x[j][e].y, wi, v[e].y);
+        }
+        fetch(j, c + i0 + j + kBatch);
+      }
+    }
+  }
+  L = warp_sum(L);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  TQ* const out = static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)head * D + 2 * lane;
+#pragma unroll
+  for (int e = 0; e < PER; e++) store2(out + 64 * e, v[e].x * inv, v[e].y * inv);
+  if (P.lse && lane == 0)
+    P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
+}
+
 template <int D>
 constexpr size_t workspace_bytes_of() {
   using C = Cfg<D>;
@@ -702,16 +763,22 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   const cudaError_t e = cudaLaunchKernelEx(&main.cfg, paged_kernel<T, TQ, D>, P);
   if (e != cudaSuccess) return e;
   const int cuts = P.by_seq ? P.B * P.groups : grid;
-  // The records that a group may be cut into: many are joined by many threads (one
-  // sequence of 8192 on 64/8 heads: 16.0 us, with two warps per query head 20.2),
-  // few by two warps (16 sequences of 150 on 16/2 heads: 8.2 us, with 16 warps 11.0).
+  // The records that a group may be cut into.  Many: 16 warps for 64 values of a query
+  // head (two sequences of 2048 on 64/8 heads, 76 records each: 10.5 us, with four warps
+  // per head 11.3, with one 17.1).  Some: four warps per query head (eight sequences,
+  // 20 records: 22.1 us, with 16 warps 28.6, with one 23.7).  Few: one warp each (64
+  // sequences of up to 1024, two or three records: 31.3 us, with four warps 34.9).
   const int64_t records = (P.cap >> P.tile_shift) < grid / cuts + 2 ? (P.cap >> P.tile_shift) : grid / cuts + 2;
-  if (records > 16) {
+  if (records > 64) {
     chpe::ServeLaunch join(dim3(cuts, P.HW * kHeads * (D / 64)), 32 * 16, 0, s);
     return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, 64, 16>, P);
   }
-  chpe::ServeLaunch join(dim3(cuts, P.HW * kHeads), 32 * 2, 0, s);
-  return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, D, 2>, P);
+  if (records > 8) {
+    chpe::ServeLaunch join(dim3(cuts, P.HW * kHeads), 32 * 4, 0, s);
+    return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, D, 4>, P);
+  }
+  chpe::ServeLaunch join(dim3(cuts, P.HW), 32 * kHeads, 0, s);
+  return cudaLaunchKernelEx(&join.cfg, combine_few_kernel<TQ, D>, P);
 }
 
 template <typename T, typename TQ>

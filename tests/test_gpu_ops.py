@@ -530,3 +530,13 @@ def test_the_same_call_gives_the_same_bits():
         out = ops.attention_decode_paged(q, tk, tv, i32(table), i32(lens), lse=lse)
         first = first or (out, lse)
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+
+
+@pytest.mark.parametrize("B, n", [(1, 9000), (2, 3000), (5, 1500), (9, 1500), (30, 400), (70, 150)])
+def test_paged_attention_joins(B, n):
+    """Sequences cut into hundreds, dozens and a few records, joined by the kernel for each."""
+    rng = np.random.default_rng(B)
+    for kind, H, KV, D in (("bf16", 8, 8, 64), ("f16", 16, 4, 256), ("f16", 8, 1, 128)):
+        lens = [int(x) for x in rng.integers(n // 2, n + 1, B)]
+        c = paged_case(rng, kind, kind, lens, H, KV, D, 16)
+        check_paged(*c[:4], lens, *c[4:], kind, kind, 16)
