@@ -60,7 +60,7 @@
 namespace {
 
 constexpr int kUnit = 16;          // positions a warp takes at a time
-constexpr int kHeads = 8;          // query heads of one warp (a "virtual" kv head)
+constexpr int kHeads = 8;          // query heads of a column operand
 constexpr int kBegin = 3;          // tiles that beginning a sequence's group costs (its query, records, refill)
 constexpr float kPShift = 14.f;    // probabilities are held times 2^14: FP16 keeps small ones
 
@@ -73,7 +73,7 @@ struct PagedLaunch {
   const int32_t* lens;
   uint32_t n_pages, page_shift;
   int32_t cap;  // positions a table row can hold
-  int32_t B, H, KV, G, HT;  // HT: virtual heads (of up to 8 query heads) per kv head
+  int32_t B, H, KV, G, HT;  // HT: virtual heads (of up to 8 N query heads) per kv head
   int32_t HW, groups;       // virtual heads of a CTA (a power of two); groups of them
   int32_t tile_shift;       // log2 of a tile's positions: 16 for each warp that shares a head
   float scale;
@@ -184,7 +184,8 @@ CHPE_DEV int tiles_of(const PagedLaunch& P, int len) { return (len + (1 << P.til
 // instead of 25.6: the CTAs with the short ones were last).
 CHPE_DEV int places_of(int tiles) { return tiles ? tiles + kBegin : 0; }
 
-template <int D>
+// N: column operands of a warp, 8 query heads each.
+template <int D, int N>
 struct Cfg {
   static constexpr int kWarps = D == 256 ? 4 : 8;
   static constexpr int kRow = D * 2;                    // bytes of a cache row of one head
@@ -192,7 +193,8 @@ struct Cfg {
   static constexpr int kStages = 3;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kSums = D * 8 + 16;              // floats that a warp hands to another of its head
-  static constexpr int kRec = kHeads * (D + 2);         // floats of a warp's record: values, then (max, sum) of each head
+  static constexpr int kWarpHeads = N * kHeads;         // query heads of a warp (a "virtual" kv head)
+  static constexpr int kRec = kWarpHeads * (D + 2);     // floats of a warp's record: values, then (max, sum) of each head
   static constexpr int kMaxCtas = D == 64 ? 320 : 160;  // grid limit, sizes the workspace
 };
 
@@ -224,9 +226,9 @@ struct Cursor {
 };
 
 // T: type of the cache; TQ: of q and out.
-template <typename T, typename TQ, int D>
-__global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
-  using C = Cfg<D>;
+template <typename T, typename TQ, int D, int N>
+__global__ void __launch_bounds__(32 * Cfg<D, N>::kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
+  using C = Cfg<D, N>;
   constexpr bool SAME = std::is_same<T, TQ>::value;  // the query is its own only part
   constexpr bool WIDE = std::is_same<T, __nv_bfloat16>::value && !SAME;
   constexpr int QP = SAME ? 1 : WIDE ? 3 : 2, PP = WIDE ? 3 : 2;  // parts of the query, of the probabilities
@@ -359,20 +361,22 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
   bool started = false;
 
   while (at.next(P, t_end)) {
-    const int vh = at.group * P.HW + hw, kvh = vh / P.HT, h0 = kvh * P.G + (vh % P.HT) * kHeads;
-    const int nh = min(kHeads, (kvh + 1) * P.G - h0);
+    const int vh = at.group * P.HW + hw, kvh = vh / P.HT, h0 = kvh * P.G + (vh % P.HT) * C::kWarpHeads;
+    const int nh = min(C::kWarpHeads, (kvh + 1) * P.G - h0);
 
-    // ---- the query's parts as column operands: lane holds head `row`
-    uint32_t qb[QP][KS][2];
-    float2 x[SAME ? 1 : KS][2];
-    {
-      const TQ* const q_row = static_cast<const TQ*>(P.q) + at.b * P.q_stride + (int64_t)(h0 + row) * D + 2 * quad;
+    // ---- the query's parts as column operands: lane holds heads `row` of each
+    uint32_t qb[N][QP][KS][2];
+    float2 x[N][SAME ? 1 : KS][2];
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+      const int head = c * kHeads + row;
+      const TQ* const q_row = static_cast<const TQ*>(P.q) + at.b * P.q_stride + (int64_t)(h0 + head) * D + 2 * quad;
 #pragma unroll
       for (int k = 0; k < KS; k++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          if constexpr (SAME) qb[0][k][h] = row < nh ? *reinterpret_cast<const uint32_t*>(q_row + k * 16 + h * 8) : 0u;
-          else x[k][h] = row < nh ? load2(q_row + k * 16 + h * 8) : make_float2(0.f, 0.f);
+          if constexpr (SAME) qb[c][0][k][h] = head < nh ? *reinterpret_cast<const uint32_t*>(q_row + k * 16 + h * 8) : 0u;
+          else x[c][k][h] = head < nh ? load2(q_row + k * 16 + h * 8) : make_float2(0.f, 0.f);
         }
     }
     if (!started) {  // the first copies, behind the query's loads
@@ -380,45 +384,54 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
       for (int i = 0; i < C::kStages - 1; i++) step_ahead();
       started = true;
     }
-    float scale[2] = {P.scale * 1.44269504088896340736f, 0.f};  // scores in powers of two
-    if constexpr (!SAME) {
-      float top = 0.f;
+    float scale[N][2];
 #pragma unroll
-      for (int k = 0; k < KS; k++)
+    for (int c = 0; c < N; c++) {
+      float mine = P.scale * 1.44269504088896340736f;  // scores in powers of two
+      if constexpr (!SAME) {
+        float top = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; h++) top = fmaxf(top, fmaxf(fabsf(x[k][h].x), fabsf(x[k][h].y)));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // a power of two that brings the largest |q| of the head to [1, 2): FP16 parts
-      // neither overflow nor lose small heads
-      const int e = top < INFINITY ? max(-126, min(126, (int)(__float_as_uint(top) >> 23) - 127)) : 0;
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      scale[0] *= __uint_as_float((uint32_t)(127 + e) << 23);
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-      for (int k = 0; k < KS; k++)
+          for (int h = 0; h < 2; h++) top = fmaxf(top, fmaxf(fabsf(x[c][k][h].x), fabsf(x[c][k][h].y)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // a power of two that brings the largest |q| of the head to [1, 2): FP16 parts
+        // neither overflow nor lose small heads
+        const int e = top < INFINITY ? max(-126, min(126, (int)(__float_as_uint(top) >> 23) - 127)) : 0;
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        mine *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float2 y = make_float2(x[k][h].x * down, x[k][h].y * down);
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-          for (int part = 0; part < QP; part++) {
-            const uint32_t w = pack2<T>(y.x, y.y);
-            qb[part][k][h] = w;
-            const float2 f = unpack2<T>(w);
-            y.x -= f.x;
-            y.y -= f.y;
+          for (int h = 0; h < 2; h++) {
+            float2 y = make_float2(x[c][k][h].x * down, x[c][k][h].y * down);
+#pragma unroll
+            for (int part = 0; part < QP; part++) {
+              const uint32_t w = pack2<T>(y.x, y.y);
+              qb[c][part][k][h] = w;
+              const float2 f = unpack2<T>(w);
+              y.x -= f.x;
+              y.y -= f.y;
+            }
           }
-        }
+      }
+      // from here on a lane holds two heads of each operand, 2 * quad and 2 * quad + 1
+      scale[c][0] = __shfl_sync(0xffffffffu, mine, 8 * quad);
+      scale[c][1] = __shfl_sync(0xffffffffu, mine, 8 * quad + 4);
     }
-    // from here on a lane holds two heads, 2 * quad and 2 * quad + 1
-    scale[1] = __shfl_sync(0xffffffffu, scale[0], 8 * quad + 4);
-    scale[0] = __shfl_sync(0xffffffffu, scale[0], 8 * quad);
 
-    float o[KS][4];  // [16 dimensions][dimension row, head], [.. + 8]
+    float o[N][KS][4];  // [16 dimensions][dimension row, head], [.. + 8]
+    float m[N][2], l[N][2];
 #pragma unroll
-    for (int t = 0; t < KS; t++)
+    for (int c = 0; c < N; c++) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[t][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int t = 0; t < KS; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[c][t][e] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; h++) m[c][h] = -INFINITY, l[c][h] = 0.f;
+    }
 
     // ldmatrix rows.  K: matrices (positions 0-7, dimensions 0-7), (8-15, 0-7), (0-7,
     // 8-15), (8-15, 8-15).  V, transposed: (positions 0-7, dimensions 0-7), (0-7,
@@ -434,105 +447,116 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
       __syncwarp();
       if (p < at.len && (ok_bits >> st & 1u)) {
         const uint32_t kb = ring + st * C::kStageBytes, vb = kb + kUnit * C::kRow;
-        float acc[2][4] = {};  // two chains: even and odd steps
+        float acc[N][2][4] = {};  // two chains: even and odd steps
 #pragma unroll
         for (int k = 0; k < KS; k++) {
           uint32_t kf[4];
           ldsm4(kf, kb + k_row * C::kRow + (((2 * k + k_ch) ^ (k_row & 7)) << 4));
 #pragma unroll
-          for (int part = 0; part < QP; part++) mma16816<T>(acc[k & 1], kf, qb[part][k][0], qb[part][k][1]);
+          for (int c = 0; c < N; c++)
+#pragma unroll
+            for (int part = 0; part < QP; part++) mma16816<T>(acc[c][k & 1], kf, qb[c][part][k][0], qb[c][part][k][1]);
         }
         // scores of positions p + row and p + row + 8, heads 2 quad and 2 quad + 1
         const bool in0 = p + row < at.len, in1 = p + row + 8 < at.len;
-        float sc[4], mn[2];
+        uint32_t pb[N][PP][2];
 #pragma unroll
-        for (int e = 0; e < 4; e++) sc[e] = (e < 2 ? in0 : in1) ? (acc[0][e] + acc[1][e]) * scale[e & 1] : -INFINITY;
+        for (int c = 0; c < N; c++) {
+          float sc[4], mn[2];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float mx = fmaxf(sc[h], sc[h + 2]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mn[h] = fmaxf(m[h], mx);
-        }
-        if (__any_sync(0xffffffffu, mn[0] != m[0] || mn[1] != m[1])) {
-          float corr[2];
+          for (int e = 0; e < 4; e++)
+            sc[e] = (e < 2 ? in0 : in1) ? (acc[c][0][e] + acc[c][1][e]) * scale[c][e & 1] : -INFINITY;
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            corr[h] = mn[h] == -INFINITY ? 1.f : exp2f(m[h] - mn[h]);
-            l[h] *= corr[h];
-            m[h] = mn[h];
+            float mx = fmaxf(sc[h], sc[h + 2]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mn[h] = fmaxf(m[c][h], mx);
+          }
+          if (__any_sync(0xffffffffu, mn[0] != m[c][0] || mn[1] != m[c][1])) {
+            float corr[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              corr[h] = mn[h] == -INFINITY ? 1.f : exp2f(m[c][h] - mn[h]);
+              l[c][h] *= corr[h];
+              m[c][h] = mn[h];
+            }
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) o[c][t][e] *= corr[e & 1];
+          }
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            y[e] = exp2f(sc[e] - ((m[c][e & 1] == -INFINITY ? 0.f : m[c][e & 1]) - kPShift));
+            l[c][e & 1] += y[e];
           }
 #pragma unroll
-          for (int t = 0; t < KS; t++)
+          for (int part = 0; part < PP; part++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[t][e] *= corr[e & 1];
+            for (int i = 0; i < 2; i++) {  // positions 0-7 and 8-15
+              const uint32_t w = pack2<T>(y[2 * i], y[2 * i + 1]);
+              pb[c][part][i] = transpose8(w);
+              const float2 f = unpack2<T>(w);
+              y[2 * i] -= f.x;
+              y[2 * i + 1] -= f.y;
+            }
         }
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          y[e] = exp2f(sc[e] - ((m[e & 1] == -INFINITY ? 0.f : m[e & 1]) - kPShift));
-          l[e & 1] += y[e];
-        }
-        uint32_t pb[PP][2];
-#pragma unroll
-        for (int part = 0; part < PP; part++)
-#pragma unroll
-          for (int i = 0; i < 2; i++) {  // positions 0-7 and 8-15
-            const uint32_t w = pack2<T>(y[2 * i], y[2 * i + 1]);
-            pb[part][i] = transpose8(w);
-            const float2 f = unpack2<T>(w);
-            y[2 * i] -= f.x;
-            y[2 * i + 1] -= f.y;
-          }
 #pragma unroll
         for (int t = 0; t < KS; t++) {
           uint32_t vf[4];
           ldsm4t(vf, vb + v_row * C::kRow + (((2 * t + v_ch) ^ (v_row & 7)) << 4));
 #pragma unroll
-          for (int part = 0; part < PP; part++) mma16816<T>(o[t], vf, pb[part][0], pb[part][1]);
+          for (int c = 0; c < N; c++)
+#pragma unroll
+            for (int part = 0; part < PP; part++) mma16816<T>(o[c][t], vf, pb[c][part][0], pb[c][part][1]);
         }
       }
       __syncwarp();  // the stage may be filled again
       st = st + 1 < C::kStages ? st + 1 : 0;
     }
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
-    }
-    if (subs > 1) {  // warps that share the head: the first one takes the others' sums
-      float* const sums = reinterpret_cast<float*>(smem + C::kRing) + hw * C::kSums;
-      __syncthreads();  // the sums of the part before are taken
-      if (sub > 0) {
-        float* const to = sums + (sub - 1) * P.HW * C::kSums;  // four per lane and 16 dimensions, then m and l
+    for (int c = 0; c < N; c++) {
 #pragma unroll
-        for (int t = 0; t < KS; t++)
-          *reinterpret_cast<float4*>(to + t * 128 + 4 * lane) = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
-        if (row == 0) *reinterpret_cast<float4*>(to + D * 8 + 4 * quad) = make_float4(m[0], m[1], l[0], l[1]);
+      for (int h = 0; h < 2; h++) {
+        l[c][h] += __shfl_xor_sync(0xffffffffu, l[c][h], 4);
+        l[c][h] += __shfl_xor_sync(0xffffffffu, l[c][h], 8);
+        l[c][h] += __shfl_xor_sync(0xffffffffu, l[c][h], 16);
       }
-      __syncthreads();
-      if (sub == 0) {
-        for (int w = 0; w < subs - 1; w++) {
-          const float* const from = sums + w * P.HW * C::kSums;
-          const float4 ml = *reinterpret_cast<const float4*>(from + D * 8 + 4 * quad);
-          float fa[2], fb[2];
+      if (subs > 1) {  // warps that share the head: the first one takes the others' sums
+        float* const sums = reinterpret_cast<float*>(smem + C::kRing) + hw * C::kSums;
+        __syncthreads();  // the sums handed over before are taken
+        if (sub > 0) {
+          float* const to = sums + (sub - 1) * P.HW * C::kSums;  // four per lane and 16 dimensions, then m and l
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const float mb = h ? ml.y : ml.x, top = fmaxf(m[h], mb);
-            fa[h] = m[h] == -INFINITY ? 0.f : exp2f(m[h] - top);
-            fb[h] = mb == -INFINITY ? 0.f : exp2f(mb - top);
-            l[h] = l[h] * fa[h] + (h ? ml.w : ml.z) * fb[h];
-            m[h] = top;
-          }
+          for (int t = 0; t < KS; t++)
+            *reinterpret_cast<float4*>(to + t * 128 + 4 * lane) = make_float4(o[c][t][0], o[c][t][1], o[c][t][2], o[c][t][3]);
+          if (row == 0) *reinterpret_cast<float4*>(to + D * 8 + 4 * quad) = make_float4(m[c][0], m[c][1], l[c][0], l[c][1]);
+        }
+        __syncthreads();
+        if (sub == 0) {
+          for (int w = 0; w < subs - 1; w++) {
+            const float* const from = sums + w * P.HW * C::kSums;
+            const float4 ml = *reinterpret_cast<const float4*>(from + D * 8 + 4 * quad);
+            float fa[2], fb[2];
 #pragma unroll
-          for (int t = 0; t < KS; t++) {
-            const float4 v = *reinterpret_cast<const float4*>(from + t * 128 + 4 * lane);
-            o[t][0] = o[t][0] * fa[0] + v.x * fb[0];
-            o[t][1] = o[t][1] * fa[1] + v.y * fb[1];
-            o[t][2] = o[t][2] * fa[0] + v.z * fb[0];
-            o[t][3] = o[t][3] * fa[1] + v.w * fb[1];
+            for (int h = 0; h < 2; h++) {
+              const float mb = h ? ml.y : ml.x, top = fmaxf(m[c][h], mb);
+              fa[h] = m[c][h] == -INFINITY ? 0.f : exp2f(m[c][h] - top);
+              fb[h] = mb == -INFINITY ? 0.f : exp2f(mb - top);
+              l[c][h] = l[c][h] * fa[h] + (h ? ml.w : ml.z) * fb[h];
+              m[c][h] = top;
+            }
+#pragma unroll
+            for (int t = 0; t < KS; t++) {
+              const float4 v = *reinterpret_cast<const float4*>(from + t * 128 + 4 * lane);
+              o[c][t][0] = o[c][t][0] * fa[0] + v.x * fb[0];
+              o[c][t][1] = o[c][t][1] * fa[1] + v.y * fb[1];
+              o[c][t][2] = o[c][t][2] * fa[0] + v.z * fb[0];
+              o[c][t][3] = o[c][t][3] * fa[1] + v.w * fb[1];
+            }
           }
         }
       }
@@ -541,40 +565,43 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
       const bool whole = at.n_tiles == at.tiles;
       float* const rec = P.part + (((size_t)2 * cta + (at.tile0 == 0 ? 1 : 0)) * P.HW + hw) * C::kRec;
       TQ* const out = static_cast<TQ*>(P.out) + at.b * P.out_stride + (int64_t)h0 * D;
-      float inv[2];
 #pragma unroll
-      for (int h = 0; h < 2; h++) inv[h] = !whole ? 1.f : l[h] == 0.f ? 0.f : 1.f / l[h];
-      // lanes of neighbouring rows swap a value, so that each has two dimensions of one head
-      const int head = 2 * quad + (row & 1), dim = row & ~1;
+      for (int c = 0; c < N; c++) {
+        float inv[2];
 #pragma unroll
-      for (int t = 0; t < KS; t++)
+        for (int h = 0; h < 2; h++) inv[h] = !whole ? 1.f : l[c][h] == 0.f ? 0.f : 1.f / l[c][h];
+        // lanes of neighbouring rows swap a value, so that each has two dimensions of one head
+        const int head = c * kHeads + 2 * quad + (row & 1), dim = row & ~1;
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const float v0 = o[t][e] * inv[0], v1 = o[t][e + 1] * inv[1];
-          const float got = __shfl_xor_sync(0xffffffffu, row & 1 ? v0 : v1, 4);
-          o[t][e] = row & 1 ? got : v0;
-          o[t][e + 1] = row & 1 ? v1 : got;
+        for (int t = 0; t < KS; t++)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float v0 = o[c][t][e] * inv[0], v1 = o[c][t][e + 1] * inv[1];
+            const float got = __shfl_xor_sync(0xffffffffu, row & 1 ? v0 : v1, 4);
+            o[c][t][e] = row & 1 ? got : v0;
+            o[c][t][e + 1] = row & 1 ? v1 : got;
+          }
+        if (head < nh) {
+          if (whole) {
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) store2(out + head * D + t * 16 + e * 4 + dim, o[c][t][e], o[c][t][e + 1]);
+          } else {
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+              for (int e = 0; e < 4; e += 2)
+                *reinterpret_cast<float2*>(rec + head * D + t * 16 + e * 4 + dim) = make_float2(o[c][t][e], o[c][t][e + 1]);
+          }
         }
-      if (head < nh) {
-        if (whole) {
-#pragma unroll
-          for (int t = 0; t < KS; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) store2(out + head * D + t * 16 + e * 4 + dim, o[t][e], o[t][e + 1]);
-        } else {
-#pragma unroll
-          for (int t = 0; t < KS; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e += 2)
-              *reinterpret_cast<float2*>(rec + head * D + t * 16 + e * 4 + dim) = make_float2(o[t][e], o[t][e + 1]);
+        if (row < 2 && head < nh) {
+          const float mh = row ? m[c][1] : m[c][0], lh = row ? l[c][1] : l[c][0];
+          if (!whole) *reinterpret_cast<float2*>(rec + C::kWarpHeads * D + 2 * head) = make_float2(mh, lh);
+          else if (P.lse)
+            P.lse[(int64_t)at.b * P.H + h0 + head] =
+                lh == 0.f ? -INFINITY : 0.693147180559945309417f * (mh + (log2f(lh) - kPShift));
         }
-      }
-      if (row < 2 && head < nh) {
-        const float mh = row ? m[1] : m[0], lh = row ? l[1] : l[0];
-        if (!whole) *reinterpret_cast<float2*>(rec + kHeads * D + 2 * head) = make_float2(mh, lh);
-        else if (P.lse)
-          P.lse[(int64_t)at.b * P.H + h0 + head] =
-              lh == 0.f ? -INFINITY : 0.693147180559945309417f * (mh + (log2f(lh) - kPShift));
       }
     }
     if (at.tile0 == 0) {
@@ -596,9 +623,9 @@ __global__ void __launch_bounds__(32 * Cfg<D>::kWarps) paged_kernel(const __grid
 // query head within the group and the DB of its D values, JW warps.  The records' weights
 // are worked out once, side by side; 4 * DB bytes of a record take DB/4 lanes, and every
 // lane has kBatch records' loads in flight.
-template <typename TQ, int D, int DB, int JW>
+template <typename TQ, int D, int N, int DB, int JW>
 __global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant__ PagedLaunch P) {
-  using C = Cfg<D>;
+  using C = Cfg<D, N>;
   constexpr int kLanes = DB / 4, kRows = 32 * JW / kLanes;  // lanes of a record, records side by side
   constexpr int kBatch = 8, kMax = C::kMaxCtas;
   static_assert(32 * JW % kLanes == 0, "");
@@ -611,8 +638,8 @@ __global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant_
   const int n = cut.z;  // at most one record per CTA
   if (n == 0) return;
   const int slice = blockIdx.y % (D / DB), hh = blockIdx.y / (D / DB);
-  const int hw = hh / kHeads, h = hh % kHeads, vh = cut.y * P.HW + hw;
-  const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * kHeads + h;
+  const int hw = hh / C::kWarpHeads, h = hh % C::kWarpHeads, vh = cut.y * P.HW + hw;
+  const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * C::kWarpHeads + h;
   if (head >= (kvh + 1) * P.G) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int my_row = tid / kLanes, col = slice * DB + 4 * (tid % kLanes);
@@ -631,7 +658,7 @@ __global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant_
 #pragma unroll
   for (int j = 0; j < PER; j++) {
     const int i = tid + j * 32 * JW;
-    ml[j] = i < n ? *reinterpret_cast<const float2*>(rec(i) + kHeads * D + 2 * h) : make_float2(-INFINITY, 0.f);
+    ml[j] = i < n ? *reinterpret_cast<const float2*>(rec(i) + C::kWarpHeads * D + 2 * h) : make_float2(-INFINITY, 0.f);
     M = fmaxf(M, ml[j].x);
   }
   M = warp_max(M);
@@ -679,12 +706,12 @@ __global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant_
     P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
 }
 
-// The same where a group is cut into a few records only: a warp per query head, 8
-// heads to a CTA, no barrier.  blockIdx.x the desc entry, blockIdx.y the head's warp of
+// The same where a group is cut into a few records only: a warp per query head, a
+// record's heads to a CTA, no barrier.  blockIdx.x the desc entry, blockIdx.y the head's warp of
 // the main kernel.
-template <typename TQ, int D>
-__global__ void __launch_bounds__(32 * kHeads) combine_few_kernel(const __grid_constant__ PagedLaunch P) {
-  using C = Cfg<D>;
+template <typename TQ, int D, int N>
+__global__ void __launch_bounds__(32 * N * kHeads) combine_few_kernel(const __grid_constant__ PagedLaunch P) {
+  using C = Cfg<D, N>;
   constexpr int PER = D / 64, kBatch = D == 256 ? 4 : 8;  // pairs of a lane, records in flight
   pdl_wait();
   pdl_launch_dependents();
@@ -692,7 +719,7 @@ __global__ void __launch_bounds__(32 * kHeads) combine_few_kernel(const __grid_c
   const int n = cut.z;
   if (n == 0) return;
   const int hw = blockIdx.y, h = threadIdx.x >> 5, lane = threadIdx.x & 31, vh = cut.y * P.HW + hw;
-  const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * kHeads + h;
+  const int kvh = vh / P.HT, head = kvh * P.G + (vh % P.HT) * C::kWarpHeads + h;
   if (head >= (kvh + 1) * P.G) return;
   auto rec = [&](int i) { return P.part + (((size_t)2 * (cut.w + i) + (i == 0 ? 1 : 0)) * P.HW + hw) * C::kRec; };
   float2 x[kBatch][PER];
@@ -704,7 +731,7 @@ __global__ void __launch_bounds__(32 * kHeads) combine_few_kernel(const __grid_c
 #pragma unroll
   for (int j = 0; j < kBatch; j++) fetch(j, j);
   float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, rec(i)[kHeads * D + 2 * h]);
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, rec(i)[C::kWarpHeads * D + 2 * h]);
   M = warp_max(M);
   float2 v[PER];
 #pragma unroll
@@ -713,7 +740,7 @@ __global__ void __launch_bounds__(32 * kHeads) combine_few_kernel(const __grid_c
   for (int c = 0; c < n; c += 32) {  // 32 records' weights at a time
     float w = 0.f;
     if (c + lane < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(rec(c + lane) + kHeads * D + 2 * h);
+      const float2 ml = *reinterpret_cast<const float2*>(rec(c + lane) + C::kWarpHeads * D + 2 * h);
       w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
       L = fmaf(ml.y, w, L);  // a NaN sum stays
     }
@@ -742,13 +769,13 @@ __global__ void __launch_bounds__(32 * kHeads) combine_few_kernel(const __grid_c
 
 template <int D>
 constexpr size_t workspace_bytes_of() {
-  using C = Cfg<D>;
+  using C = Cfg<D, D == 128 ? 2 : 1>;
   return C::kMaxCtas * sizeof(int4) + (size_t)2 * C::kMaxCtas * C::kWarps * C::kRec * sizeof(float);
 }
 
-template <typename T, typename TQ, int D>
+template <typename T, typename TQ, int D, int N>
 cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
-  using C = Cfg<D>;
+  using C = Cfg<D, N>;
   // per device: SMs times resident CTAs of this kernel (one query, then kept)
   static int grid_of[64] = {};
   const int dev = device >= 0 && device < 64 ? device : -1;
@@ -756,10 +783,10 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   if (grid == 0) {
     int sms = 0, res = 0;
     const int most = C::kRing + (C::kWarps - 1) * C::kSums * (int)sizeof(float);  // one head: all other warps hand over
-    cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, TQ, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    cudaError_t e = cudaFuncSetAttribute(paged_kernel<T, TQ, D, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess)
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, TQ, D>, 32 * C::kWarps, most);
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&res, paged_kernel<T, TQ, D, N>, 32 * C::kWarps, most);
     if (e != cudaSuccess) return e;
     grid = sms * (res < 1 ? 1 : res);
     if (grid > C::kMaxCtas) grid = C::kMaxCtas;
@@ -770,7 +797,7 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   P.desc = static_cast<int4*>(workspace);
   P.part = reinterpret_cast<float*>(P.desc + C::kMaxCtas);
   chpe::ServeLaunch main(dim3(grid), 32 * C::kWarps, C::kRing + (subs - 1) * P.HW * C::kSums * sizeof(float), s);
-  const cudaError_t e = cudaLaunchKernelEx(&main.cfg, paged_kernel<T, TQ, D>, P);
+  const cudaError_t e = cudaLaunchKernelEx(&main.cfg, paged_kernel<T, TQ, D, N>, P);
   if (e != cudaSuccess) return e;
   const int cuts = P.by_seq ? P.B * P.groups : grid;
   // The records that a group may be cut into.  Many: 16 warps for 64 values of a query
@@ -780,22 +807,22 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   // sequences of up to 1024, two or three records: 31.3 us, with four warps 34.9).
   const int64_t records = (P.cap >> P.tile_shift) < grid / cuts + 2 ? (P.cap >> P.tile_shift) : grid / cuts + 2;
   if (records > 64) {
-    chpe::ServeLaunch join(dim3(cuts, P.HW * kHeads * (D / 64)), 32 * 16, 0, s);
-    return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, 64, 16>, P);
+    chpe::ServeLaunch join(dim3(cuts, P.HW * C::kWarpHeads * (D / 64)), 32 * 16, 0, s);
+    return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, N, 64, 16>, P);
   }
   if (records > 8) {
-    chpe::ServeLaunch join(dim3(cuts, P.HW * kHeads), 32 * 4, 0, s);
-    return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, D, 4>, P);
+    chpe::ServeLaunch join(dim3(cuts, P.HW * C::kWarpHeads), 32 * 4, 0, s);
+    return cudaLaunchKernelEx(&join.cfg, combine_kernel<TQ, D, N, D, 4>, P);
   }
-  chpe::ServeLaunch join(dim3(cuts, P.HW), 32 * kHeads, 0, s);
-  return cudaLaunchKernelEx(&join.cfg, combine_few_kernel<TQ, D>, P);
+  chpe::ServeLaunch join(dim3(cuts, P.HW), 32 * C::kWarpHeads, 0, s);
+  return cudaLaunchKernelEx(&join.cfg, combine_few_kernel<TQ, D, N>, P);
 }
 
 template <typename T, typename TQ>
-cudaError_t launch_d(const PagedLaunch& P, void* workspace, uint32_t d, int device, cudaStream_t s) {
-  if (d == 64) return launch<T, TQ, 64>(P, workspace, device, s);
-  if (d == 128) return launch<T, TQ, 128>(P, workspace, device, s);
-  return launch<T, TQ, 256>(P, workspace, device, s);
+cudaError_t launch_d(const PagedLaunch& P, void* workspace, uint32_t d, int operands, int device, cudaStream_t s) {
+  if (d == 64) return launch<T, TQ, 64, 1>(P, workspace, device, s);
+  if (d == 256) return launch<T, TQ, 256, 1>(P, workspace, device, s);
+  return operands == 2 ? launch<T, TQ, 128, 2>(P, workspace, device, s) : launch<T, TQ, 128, 1>(P, workspace, device, s);
 }
 
 }  // namespace
@@ -863,9 +890,17 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   P.cap = (int32_t)(cap < INT32_MAX - 1024 ? cap : INT32_MAX - 1024);
   P.B = (int32_t)batch, P.H = (int32_t)num_heads, P.KV = (int32_t)num_kv_heads;
   P.G = P.H / P.KV;
-  P.HT = (P.G + kHeads - 1) / kHeads;
-  const int vh = P.KV * P.HT, warps = head_dim == 256 ? Cfg<256>::kWarps : Cfg<128>::kWarps;
-  static_assert(Cfg<64>::kWarps == Cfg<128>::kWarps, "");
+  // More than 8 query heads per kv head: two operands per warp, so that the rows copied
+  // serve 16, or two warps that copy the same rows.  At heads of 128 the former takes 72
+  // instead of 82 us for 64 sequences of up to 8192 on 64/4 heads, but 11.4 instead of
+  // 9.8 for one of 4000 on 32/2, so it is taken where the tables have room for 64 MB of
+  // entries; at 64 they are even (26.9 us), and at 256 the registers are lacking.
+  const int64_t room = (int64_t)batch * P.cap * num_kv_heads * head_dim * 4;
+  const int operands = head_dim == 128 && P.G > kHeads && room >= (64 << 20) ? 2 : 1;
+  const int per_warp = operands * kHeads;
+  P.HT = (P.G + per_warp - 1) / per_warp;
+  const int vh = P.KV * P.HT, warps = head_dim == 256 ? Cfg<256, 1>::kWarps : Cfg<128, 1>::kWarps;
+  static_assert(Cfg<64, 1>::kWarps == Cfg<128, 1>::kWarps, "");
   P.HW = warps;
   while (vh % P.HW != 0) P.HW /= 2;
   P.groups = vh / P.HW;
@@ -878,10 +913,10 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   chpe::DeviceScope scope(c.launch_device());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (cache_dtype == CHPE_F16) e = dtype == CHPE_F32 ? launch_d<__half, float>(P, workspace, head_dim, c.device, s)
-                                                     : launch_d<__half, __half>(P, workspace, head_dim, c.device, s);
-  else e = dtype == CHPE_F32 ? launch_d<__nv_bfloat16, float>(P, workspace, head_dim, c.device, s)
-                             : launch_d<__nv_bfloat16, __nv_bfloat16>(P, workspace, head_dim, c.device, s);
+  if (cache_dtype == CHPE_F16) e = dtype == CHPE_F32 ? launch_d<__half, float>(P, workspace, head_dim, operands, c.device, s)
+                                                     : launch_d<__half, __half>(P, workspace, head_dim, operands, c.device, s);
+  else e = dtype == CHPE_F32 ? launch_d<__nv_bfloat16, float>(P, workspace, head_dim, operands, c.device, s)
+                             : launch_d<__nv_bfloat16, __nv_bfloat16>(P, workspace, head_dim, operands, c.device, s);
   if (e != cudaSuccess) {
     snprintf(c.msg, sizeof(c.msg), "launch: %s", cudaGetErrorString(e));
     c.rc = -3;

@@ -143,7 +143,8 @@ def check_paged(q, tk, tv, table, lens, xq, xk, xv, kind, cache, page, scale=Non
 
 
 @pytest.mark.parametrize("kind, cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
-@pytest.mark.parametrize("H, KV, D", [(16, 2, 128), (16, 4, 256), (4, 4, 64), (12, 4, 128), (24, 2, 64), (9, 1, 256)])
+@pytest.mark.parametrize("H, KV, D", [(16, 2, 128), (16, 4, 256), (4, 4, 64), (12, 4, 128), (24, 2, 64), (9, 1, 256), (64, 4, 128),
+                                      (40, 2, 64), (33, 1, 128)])
 @pytest.mark.parametrize("page", [16, 64])
 def test_paged_attention(kind, cache, H, KV, D, page):
     rng = np.random.default_rng(H + D + page)
@@ -536,7 +537,19 @@ def test_the_same_call_gives_the_same_bits():
 def test_paged_attention_joins(B, n):
     """Sequences cut into hundreds, dozens and a few records, joined by the kernel for each."""
     rng = np.random.default_rng(B)
-    for kind, H, KV, D in (("bf16", 8, 8, 64), ("f16", 16, 4, 256), ("f16", 8, 1, 128)):
+    for kind, H, KV, D in (("bf16", 8, 8, 64), ("f16", 16, 4, 256), ("f16", 8, 1, 128), ("bf16", 24, 2, 64)):
         lens = [int(x) for x in rng.integers(n // 2, n + 1, B)]
         c = paged_case(rng, kind, kind, lens, H, KV, D, 16)
         check_paged(*c[:4], lens, *c[4:], kind, kind, 16)
+
+
+@pytest.mark.parametrize("kind, cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("H, KV", [(12, 1), (32, 2), (33, 1), (60, 4)])
+def test_paged_attention_many_heads_per_kv_head_and_wide_tables(kind, cache, H, KV):
+    """More than 8 query heads per kv head behind tables with room for long sequences."""
+    rng = np.random.default_rng(H)
+    lens = [700, 0, 16, 333, 1]
+    q, tk, tv, table, xq, xk, xv = paged_case(rng, kind, cache, lens, H, KV, 128, 64)
+    room = np.full((5, 64 * 2 ** 20 // (5 * 64 * KV * 128 * 4) + 1), -1, np.int32)
+    room[:, :table.shape[1]] = table
+    check_paged(q, tk, tv, room, lens, xq, xk, xv, kind, cache, 64)
