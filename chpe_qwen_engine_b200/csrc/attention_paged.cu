@@ -895,8 +895,8 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   // instead of 82 us for 64 sequences of up to 8192 on 64/4 heads, but 11.4 instead of
   // 9.8 for one of 4000 on 32/2, so it is taken where the tables have room for 64 MB of
   // entries; at 64 they are even (26.9 us), and at 256 the registers are lacking.
-  const int64_t room = (int64_t)batch * P.cap * num_kv_heads * head_dim * 4;
-  const int operands = head_dim == 128 && P.G > kHeads && room >= (64 << 20) ? 2 : 1;
+  const double room = 4.0 * batch * P.cap * num_kv_heads * head_dim;
+  const int operands = head_dim == 128 && P.G > kHeads && room >= 64.0 * (1 << 20) ? 2 : 1;
   const int per_warp = operands * kHeads;
   P.HT = (P.G + per_warp - 1) / per_warp;
   const int vh = P.KV * P.HT, warps = head_dim == 256 ? Cfg<256, 1>::kWarps : Cfg<128, 1>::kWarps;
