@@ -225,11 +225,13 @@ __global__ void __launch_bounds__(32 * kWarps) qk_rope_kernel(const __grid_const
             b[e] = b[e] * inv * wb[e];
           }
         }
+        if (sub < sh) {  // the others' values stay as they are, infinities and signs of zero too
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float x = a[e], y = b[e];
-          a[e] = fmaf(x, r[e].x, -y * r[e].y);
-          b[e] = fmaf(y, r[e].x, x * r[e].y);
+          for (int e = 0; e < 8; e++) {
+            const float x = a[e], y = b[e];
+            a[e] = fmaf(x, r[e].x, -y * r[e].y);
+            b[e] = fmaf(y, r[e].x, x * r[e].y);
+          }
         }
       }
       if (h.x >= (h.y == 0 ? P.H : P.KV)) continue;

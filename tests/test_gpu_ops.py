@@ -98,6 +98,23 @@ def test_qk_values_at_the_type_limits():
     assert torch.equal(out, k)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D, rope", [(64, 0), (64, 32), (128, 48), (256, 64)])
+def test_qk_what_is_not_rotated_stays(kind, D, rope):
+    """Bit for bit, whatever stands beside it: infinities, NaN, zeros of both signs."""
+    x = np.random.default_rng(D).standard_normal((3, 2, D)).astype(np.float32)
+    x[:, :, rope + 1::7], x[:, :, rope + 2::7], x[:, :, rope + 3::7] = np.inf, np.nan, -0.0
+    q, _ = put(x, kind)
+    kc, vc = (torch.zeros(1, 16, 2, D, dtype=DT["f16" if kind == "f32" else kind], device=DEV) for _ in range(2))
+    out, _ = ops.qk_norm_rope(q, q, q, i32([1, 2, 3]), ops.rope_inv_freq(1e4, rope) if rope else None, k_cache=kc, v_cache=vc,
+                              slots=torch.tensor([3, 4, 5], device=DEV))
+    bits = lambda t: t[..., rope:].contiguous().view(torch.int32 if t.dtype == torch.float32 else torch.int16)  # noqa: E731
+    number = ~torch.isnan(q[..., rope:])
+    assert torch.equal(bits(out)[number], bits(q)[number]) and torch.isnan(out[..., rope:][~number]).all()
+    row = q.to(kc.dtype)
+    assert torch.equal(bits(kc[0, 3:6])[number], bits(row)[number]) and torch.equal(bits(vc[0, 3:6])[number], bits(row)[number])
+
+
 def test_qk_more_tokens_than_a_grid_row():
     T = 70001
     q = torch.randn(T, 1, 64, device=DEV, dtype=torch.bfloat16)
