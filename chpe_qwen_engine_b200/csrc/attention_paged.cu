@@ -11,7 +11,7 @@
 // Work split.  A CTA takes several kv heads of the same positions at once, a warp
 // each, because a position's heads lie side by side in the cache: what a CTA reads
 // is then whole pages, not a 256-byte row of every 2 KB (one head per CTA
-// took 162 us instead of 124 for a batch of 64 on 64/8 heads of 128).  Where there are
+// took 162 us instead of 124, all else alike, for a batch of 64 on 64/8 heads of 128).  Where there are
 // fewer heads than warps the remaining warps take further 16-position units of
 // the tile.  The work is a line of tiles: sequence by sequence, group of heads by
 // group, tile by tile, and CTA c of C takes the c-th of C equal stretches,
@@ -29,8 +29,8 @@
 // waits for no other warp; only warps that share a head meet, at the end of a part.
 //
 // Measured (device time): 131071 positions of one sequence on 64/8 heads of 128: 92 us,
-// 91 % of the copy rate; 64 sequences of up to 8192 there: 125 us, 90 %; 37 of up
-// to 4093 on 16/4 heads of 256: 45 us, 72 %; one of 77 on 16/2 heads: 7.9 us.
+// 91 % of the copy rate; 64 sequences of up to 8192 there: 122 us, 92 %; 37 of up
+// to 4093 on 16/4 heads of 256: 43 us, 76 %; one of 77 on 16/2 heads: 7.9 us.
 // What is left: SMs get bandwidth unevenly, so that CTAs with equal shares end
 // 10 % before and after the mean, and the records' join, 3 us behind a gap of 2.
 // Handing a fifth of the line out to whoever is done evened the ends out but cost as

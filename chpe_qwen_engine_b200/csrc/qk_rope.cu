@@ -27,8 +27,8 @@
 // are goes by the number of tokens: one group per warp when there are few (a
 // single token of the 72B's heads is 20 warps), all of a token's when the tokens alone fill
 // the GPU and the angles are worth sharing.  16384 tokens of 64/8 heads of 128 in
-// BF16: 119 us, 5.6 TB/s, 87 % of the copy rate (a plain copy of q, k and v alone takes 102);
-// one token: 3.3 us, a launch and four dependent loads.
+// BF16: 115 us, 5.8 TB/s, 90 % of the copy rate (a plain copy of q, k and v alone takes 102);
+// one token: 2.9 us, a launch and three dependent loads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
