@@ -432,6 +432,7 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
   if (!es) return c.fail(-1, "unknown dtype %lld", dtype), c.done();
   if (vocab == 0 || vocab > 0x7fffffffu) return c.fail(-1, "vocab must be 1..2^31-1"), c.done();
   if (batch > (1u << 24)) return c.fail(-1, "batch must be at most 2^24"), c.done();
+  if (batch == 0) return c.done();
   if (!out && !argmax) return c.fail(-1, "neither out nor argmax to write"), c.done();
   if ((prompt_lens || total_lens || repetition || frequency || presence) && !history)
     return c.fail(-1, "lengths or penalties without a history"), c.done();
@@ -451,7 +452,6 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
     if (mask && mask_stride != 0 && (mask_stride < words || mask_stride > most))
       return c.fail(-1, "mask_stride must be 0 or at least %lld words", words), c.done();
   }
-  if (batch == 0) return c.done();
   c.ptr(logits, "logits", es);
   if (history && history_len) c.ptr(history, "history", 4);
   c.ptr_or_null(prompt_lens, "prompt_lens", 4);

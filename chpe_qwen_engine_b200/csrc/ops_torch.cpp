@@ -358,7 +358,9 @@ PyObject* logits_process(PyObject*, PyObject* const* args, Py_ssize_t n, PyObjec
     const int64_t ms = mask ? rows_of(*mask, "mask", at::kInt, dev, B, (V + 31) / 32) : 0;
     check(chpe_logits_process(
         x.data_ptr(), dt, xs, u32(B, "the batch"), u32(V, "the vocabulary"),
-        hist ? static_cast<const int32_t*>(hist->data_ptr()) : nullptr, hs, hist ? u32(hist->size(1), "history") : 0,
+        // (an empty history has no address of its own, but is one)
+        !hist ? nullptr : static_cast<const int32_t*>(hist->numel() ? hist->data_ptr() : x.data_ptr()), hs,
+        hist ? u32(hist->size(1), "history") : 0,
         vec<int32_t>(a.tensor(PLEN, "prompt_lens"), "prompt_lens", at::kInt, B, dev),
         vec<int32_t>(a.tensor(TLEN, "total_lens"), "total_lens", at::kInt, B, dev),
         vec<float>(a.tensor(REP, "repetition"), "repetition", at::kFloat, B, dev),

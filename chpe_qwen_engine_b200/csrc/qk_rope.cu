@@ -299,6 +299,7 @@ extern "C" int chpe_qk_norm_rope(const void* q, const void* k, const void* v, in
   if (rope_dim > head_dim || rope_dim % 16 != 0)
     return c.fail(-1, "rope_dim must be a multiple of 16 up to head_dim"), c.done();
   if (num_tokens > 0x7fffffffu) return c.fail(-1, "too many tokens"), c.done();
+  if (num_tokens == 0) return c.done();
   if (!k_cache != !v_cache) return c.fail(-1, "k_cache and v_cache go together"), c.done();
   if (!k_cache && !k_out) return c.fail(-1, "neither a cache nor k_out to write k to"), c.done();
   if (k_cache && cache_dtype != CHPE_F16 && cache_dtype != CHPE_BF16)
@@ -306,7 +307,6 @@ extern "C" int chpe_qk_norm_rope(const void* q, const void* k, const void* v, in
   if (k_cache && dtype != CHPE_F32 && dtype != cache_dtype)
     return c.fail(-1, "the cache must have the type of q, k and v unless those are float"), c.done();
   if (k_cache && cache_rows > (uint64_t)INT64_MAX) return c.fail(-1, "cache_rows is too large"), c.done();
-  if (num_tokens == 0) return c.done();
   const int64_t lane = 16 / (int64_t)es;  // elements of a 16-byte access
   const int64_t hq = (int64_t)num_heads * head_dim, hk = (int64_t)num_kv_heads * head_dim;
   const int64_t strides[5] = {q_stride, k_stride, k_cache ? v_stride : hk, q_out_stride, k_out ? k_out_stride : hk};
@@ -325,7 +325,7 @@ extern "C" int chpe_qk_norm_rope(const void* q, const void* k, const void* v, in
     const double f = inv_freq[i];
     if (!(fabs(f) <= 16.0)) return c.fail(-1, "inv_freq[%lld] is not a number within 16", i), c.done();
     long double turns = (long double)f * 0.159154943091895335768883763372514362L;
-    turns -= floorl(turns);
+    if (turns < 0.0L || turns >= 1.0L) turns -= floorl(turns);  // a library call, 1 us for 64 of them
     const long double scaled = turns * 18446744073709551616.0L + 0.5L;
     P.turn[i] = scaled >= 18446744073709551616.0L ? 0u : (uint64_t)scaled;
   }

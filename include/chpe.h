@@ -419,7 +419,8 @@ int chpe_attention_decode_paged(const void *q, int dtype, int64_t q_stride, cons
  * 65535) entries per row.  Ids outside 0..vocab-1 (-1 for unused entries) are
  * passed over in both lists.  mask [batch][mask_stride] of 32-bit words, bit v % 32
  * of word v / 32, 1: allowed.  A bias_stride or mask_stride of 0 gives all rows the
- * first one's.  history, the biases and the mask may each be NULL.
+ * first one's.  history, the biases and the mask may each be NULL; lengths and
+ * penalties need a history (of no entries, if there are none yet).
  * out [batch][out_stride] float gets every x (NULL: not wanted) and may be the
  * logits themselves where those are float with the same stride; argmax [batch]
  * (NULL: not wanted) the lowest token of the largest x: NaN never wins, and -1

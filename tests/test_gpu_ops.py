@@ -570,3 +570,31 @@ def test_paged_attention_many_heads_per_kv_head_and_wide_tables(kind, cache, H, 
     room = np.full((5, 64 * 2 ** 20 // (5 * 64 * KV * 128 * 4) + 1), -1, np.int32)
     room[:, :table.shape[1]] = table
     check_paged(q, tk, tv, room, lens, xq, xk, xv, kind, cache, 64)
+
+
+def test_paged_attention_workspace_of_any_content():
+    """Garbage in the workspace, and calls of other shapes before, change nothing."""
+    rng = np.random.default_rng(14)
+    ws = ops.attention_workspace(128, DEV)
+    for lens, H, KV in (([2500, 3, 0, 900], 16, 2), ([9] * 200, 8, 8), ([5000], 8, 1)):
+        q, tk, tv, table, *_ = paged_case(rng, "f16", "f16", lens, H, KV, 128, 32)
+        want = ops.attention_decode_paged(q, tk, tv, i32(table), i32(lens))
+        for fill in (0xFF, 0x7F, None):
+            if fill is not None:
+                ws.fill_(fill)
+            assert torch.equal(want, ops.attention_decode_paged(q, tk, tv, i32(table), i32(lens), workspace=ws))
+
+
+def test_calls_without_rows():
+    e = lambda *n, dt=torch.float16: torch.empty(*n, dtype=dt, device=DEV)  # noqa: E731
+    kc = torch.full((2, 16, 2, 64), 5.0, dtype=torch.float16, device=DEV)
+    q, k = ops.qk_norm_rope(e(0, 4, 64), e(0, 2, 64), e(0, 2, 64), e(0, dt=torch.int32), ops.rope_inv_freq(1e4, 64),
+                            k_cache=kc, v_cache=kc.clone(), slots=e(0, dt=torch.int64))
+    assert q.shape == (0, 4, 64) and k is None and (kc == 5).all()
+    assert ops.attention_decode_paged(e(0, 4, 64), kc, kc, e(0, 3, dt=torch.int32), e(0, dt=torch.int32)).shape == (0, 4, 64)
+    x, t = ops.logits_process(e(0, 100), history=e(0, 5, dt=torch.int32))
+    assert x.shape == (0, 100) and t.shape == (0,)
+    x = torch.randn(3, 100, device=DEV)
+    y, t = ops.logits_process(x, history=e(3, 0, dt=torch.int32), repetition=torch.ones(3, device=DEV),
+                              bias_ids=e(3, 0, dt=torch.int32), bias_values=e(3, 0, dt=torch.float32))
+    assert torch.equal(x, y) and torch.equal(t, x.argmax(1).int())
