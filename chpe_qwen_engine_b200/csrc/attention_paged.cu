@@ -42,9 +42,8 @@
 // sums take half the registers of the untransposed form (D=256: 64 instead of 128 per
 // lane).  P^T comes out of S^T by movmatrix.  Queries of the cache's type go in as
 // they are; float ones as two FP16 or three BF16 parts (22 and 24 bits), each a
-// column operand of its own, and so do the probabilities (two parts; three for
-// float queries over a BF16 cache), held times 2^14 so that FP16 keeps the
-// small ones.  tcgen05.mma would need its operands in shared memory or TMEM in
+// column operand of its own, and so do the probabilities, held times 2^14 so that
+// FP16 keeps the small ones.  tcgen05.mma would need its operands in shared memory or TMEM in
 // layouts of 128 rows for 8 columns of work; the tensor pipe is nearly idle either way.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -230,8 +229,8 @@ template <typename T, typename TQ, int D, int N>
 __global__ void __launch_bounds__(32 * Cfg<D, N>::kWarps) paged_kernel(const __grid_constant__ PagedLaunch P) {
   using C = Cfg<D, N>;
   constexpr bool SAME = std::is_same<T, TQ>::value;  // the query is its own only part
-  constexpr bool WIDE = std::is_same<T, __nv_bfloat16>::value && !SAME;
-  constexpr int QP = SAME ? 1 : WIDE ? 3 : 2, PP = WIDE ? 3 : 2;  // parts of the query, of the probabilities
+  // parts of the probabilities, of the query: FP16 has 22 bits in two, BF16 24 in three
+  constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 3 : 2, QP = SAME ? 1 : PP;
   constexpr int KS = D / 16, CH = D / 8;  // 16-dimension steps, 16-byte chunks per row
   constexpr int W = C::kWarps, THREADS = 32 * W;
   extern __shared__ __align__(128) unsigned char smem[];

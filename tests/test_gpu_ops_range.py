@@ -1,0 +1,55 @@
+"""The batched decode operators at the ends of their range.  References and bounds
+as in test_gpu_ops.py."""
+import numpy as np
+import pytest
+
+from test_gpu_ops import DEV, close, i32, put
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+if torch is not None:
+    from chpe_qwen_engine_b200 import ops
+
+
+# ---- precision of the attention's operands -------------------------------------------
+def bf16(x):
+    return torch.tensor(x, dtype=torch.float64).bfloat16().double().numpy()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_probabilities_keep_f32_bits_over_a_bf16_cache(kind, D):
+    """Weights 1, 1 and p with values -hi, -lo and 1, where hi + lo are the two BF16 parts of
+    p: the output is what 16 bits of p leave out."""
+    rng = np.random.default_rng(1)
+    x = np.unique(bf16(-rng.uniform(0.25, 1.0, 4000)))
+    p = np.exp(x)
+    hi = bf16(p)
+    lo = bf16(p - hi)
+    at = np.argsort(-np.abs(p - hi - lo) / p)[:8]  # those whose rest is largest
+    assert np.all(np.abs(p - hi - lo)[at] > 0.75 * 2.0 ** -18 * p[at])
+    x, p, hi, lo = x[at], p[at], hi[at], lo[at]
+    q, k, v = np.zeros((1, 8, D)), np.zeros((1, 16, 8, D)), np.zeros((1, 16, 8, D))
+    q[0, :, 0] = 1.0
+    k[0, 2, :, 0] = x
+    v[0, 0], v[0, 1], v[0, 2] = -hi[:, None], -lo[:, None], 1.0
+    tq, tk, tv = put(q, kind)[0], put(k, "bf16")[0], put(v, "bf16")[0]
+    out = ops.attention_decode_paged(tq, tk, tv, i32([[0]]), i32([3]), scale=1.0)
+    ref = ((p - hi - lo) / (2 + p))[None, :, None] * np.ones((1, 8, D))
+    # p is off by: log2 e and its product with x (2^-24 each of |x| log2 e < 1.5), the sum of
+    # the exponent's argument (half a step below 16: 2^-21), exp2 (2 ulp); the products are summed in f32, cut
+    e = np.log(2) * (1.5 * 2.0 ** -23 + 2.0 ** -21) + 2.0 ** -22 + 4 * 2.0 ** -23
+    close(out, ref, e * (2 * p / (2 + p))[None, :, None], kind)
+
+
+def test_the_longest_batch_repeats_its_bits():
+    g = torch.Generator(DEV).manual_seed(5)
+    n, page = 131071, 64
+    table = torch.randperm(2048, generator=g, device=DEV).int()[None]
+    kc, vc = (torch.randn(2048, page, 8, 128, generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, 64, 128, generator=g, device=DEV, dtype=torch.bfloat16)
+    first, lse = None, torch.empty(1, 64, device=DEV)
+    for _ in range(20):
+        out = ops.attention_decode_paged(q, kc, vc, table, i32([n]), lse=lse)
+        first = first or (out, lse.clone())
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
