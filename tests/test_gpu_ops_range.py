@@ -3,7 +3,7 @@ as in test_gpu_ops.py."""
 import numpy as np
 import pytest
 
-from test_gpu_ops import DEV, close, i32, put
+from test_gpu_ops import DEV, check_paged, close, f64, i32, paged_case, put
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -53,3 +53,28 @@ def test_the_longest_batch_repeats_its_bits():
         out = ops.attention_decode_paged(q, kc, vc, table, i32([n]), lse=lse)
         first = first or (out, lse.clone())
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("D, H, KV", [(64, 4, 2), (128, 16, 2), (256, 4, 4), (128, 32, 2)])
+@pytest.mark.parametrize("large", [1e3, 4e4, 1e6])
+def test_paged_attention_one_large_query_dimension(cache, D, H, KV, large):
+    """A dimension far above the others, which the keys do not have: the others count alone."""
+    rng = np.random.default_rng(D)
+    lens = [300, 17]
+    q, tk, tv, table, xq, xk, xv = paged_case(rng, "f32", cache, lens, H, KV, D, 16)
+    q[:, :, 5] = large
+    tk[..., 5] = 0
+    check_paged(q, tk, tv, table, lens, f64(q), f64(tk), xv, "f32", cache, 16)
+
+
+@pytest.mark.parametrize("largest", [2.0 ** 127, 2.0 ** 100, 2.0 ** -100, 2.0 ** -126, 2.0 ** -140])
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_paged_attention_queries_of_every_size(cache, largest):
+    """The scale brings the scores back to ordinary ones, as far as f32 holds it."""
+    rng = np.random.default_rng(2)
+    lens = [100]
+    q, tk, tv, table, xq, xk, xv = paged_case(rng, "f32", cache, lens, 4, 2, 64, 16)
+    q = (q / q.abs().max() * 1.5).double().mul(largest).float()
+    scale = float(np.clip(0.2 / largest, 2.0 ** -126, 1e6))
+    check_paged(q, tk, tv, table, lens, f64(q), xk, xv, "f32", cache, 16, scale=scale)
