@@ -42,8 +42,8 @@
 // sums take half the registers of the untransposed form (D=256: 64 instead of 128 per
 // lane).  P^T comes out of S^T by movmatrix.  Queries of the cache's type go in as
 // they are; float ones as two FP16 or three BF16 parts (22 and 24 bits), each a
-// column operand of its own, and so do the probabilities, held times 2^14 so that
-// FP16 keeps the small ones.  tcgen05.mma would need its operands in shared memory or TMEM in
+// column operand of its own, and so do the probabilities, held times 2^14 over
+// FP16, which keeps the small ones.  tcgen05.mma would need its operands in shared memory or TMEM in
 // layouts of 128 rows for 8 columns of work; the tensor pipe is nearly idle either way.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -61,7 +61,11 @@ namespace {
 constexpr int kUnit = 16;          // positions a warp takes at a time
 constexpr int kHeads = 8;          // query heads of a column operand
 constexpr int kBegin = 3;          // tiles that beginning a sequence's group costs (its query, records, refill)
-constexpr float kPShift = 14.f;    // probabilities are held times 2^14: FP16 keeps small ones
+// Probabilities are held times 2^kPShift: over FP16, whose parts end at 2^-24, so that small
+// ones are kept; over BF16 as they are (times 2^14, values above 2^113 of a single
+// position went beyond f32).
+template <typename T>
+constexpr float kPShift = std::is_same<T, __half>::value ? 14.f : 0.f;
 
 struct PagedLaunch {
   const void* q;
@@ -81,6 +85,7 @@ struct PagedLaunch {
   float* lse;
   float* part;  // records [2 * grid][HW]
   int4* desc;   // cuts: sequence, group, number of CTAs (0: not cut), the first of them
+  float p_shift;   // kPShift of the cache's type
   int32_t by_seq;  // a desc entry for each sequence and group (they are at most `grid`); else for each CTA
 };
 
@@ -492,7 +497,7 @@ __global__ void __launch_bounds__(32 * Cfg<D, N>::kWarps) paged_kernel(const __g
           float y[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            y[e] = exp2f(sc[e] - ((m[c][e & 1] == -INFINITY ? 0.f : m[c][e & 1]) - kPShift));
+            y[e] = exp2f(sc[e] - ((m[c][e & 1] == -INFINITY ? 0.f : m[c][e & 1]) - kPShift<T>));
             l[c][e & 1] += y[e];
           }
 #pragma unroll
@@ -602,7 +607,7 @@ __global__ void __launch_bounds__(32 * Cfg<D, N>::kWarps) paged_kernel(const __g
           if (!whole) *reinterpret_cast<float2*>(rec + C::kWarpHeads * D + 2 * head) = make_float2(mh, lh);
           else if (P.lse)
             P.lse[(int64_t)at.b * P.H + h0 + head] =
-                lh == 0.f ? -INFINITY : 0.693147180559945309417f * (mh + (log2f(lh) - kPShift));
+                lh == 0.f ? -INFINITY : 0.693147180559945309417f * (mh + (log2f(lh) - kPShift<T>));
         }
       }
     }
@@ -705,7 +710,7 @@ __global__ void __launch_bounds__(32 * JW) combine_kernel(const __grid_constant_
     store1(static_cast<TQ*>(P.out) + cut.x * P.out_stride + (int64_t)head * D + slice * DB + d, L == 0.f ? 0.f : y / L);
   }
   if (P.lse && tid == 0 && slice == 0)
-    P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
+    P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - P.p_shift));
 }
 
 // The same where a group is cut into a few records only: a warp per query head, a
@@ -766,7 +771,7 @@ __global__ void __launch_bounds__(32 * N * kHeads) combine_few_kernel(const __gr
 #pragma unroll
   for (int e = 0; e < PER; e++) store2(out + 64 * e, v[e].x * inv, v[e].y * inv);
   if (P.lse && lane == 0)
-    P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - kPShift));
+    P.lse[(int64_t)cut.x * P.H + head] = L == 0.f ? -INFINITY : 0.693147180559945309417f * (M + (log2f(L) - P.p_shift));
 }
 
 template <int D>
@@ -795,6 +800,7 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
     if (dev >= 0) __atomic_store_n(&grid_of[dev], grid, __ATOMIC_RELAXED);
   }
   const int subs = C::kWarps / P.HW;
+  P.p_shift = kPShift<T>;
   P.by_seq = (int64_t)P.B * P.groups <= grid;
   P.desc = static_cast<int4*>(workspace);
   P.part = reinterpret_cast<float*>(P.desc + C::kMaxCtas);

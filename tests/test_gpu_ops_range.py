@@ -78,3 +78,13 @@ def test_paged_attention_queries_of_every_size(cache, largest):
     q = (q / q.abs().max() * 1.5).double().mul(largest).float()
     scale = float(np.clip(0.2 / largest, 2.0 ** -126, 1e6))
     check_paged(q, tk, tv, table, lens, f64(q), xk, xv, "f32", cache, 16, scale=scale)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("lens, H, KV, D", [([100, 7], 8, 2, 128), ([2000], 4, 4, 64), ([2000], 8, 2, 256), ([600] * 30, 8, 8, 128)])
+def test_paged_attention_large_bf16_values(kind, lens, H, KV, D):
+    """Values of 2^112 over some thousand positions: their sums are within f32."""
+    rng = np.random.default_rng(3)
+    q, tk, tv, table, xq, xk, xv = paged_case(rng, kind, "bf16", lens, H, KV, D, 16)
+    tv = tv * 2.0 ** 112
+    check_paged(q, tk, tv, table, lens, xq, xk, f64(tv), kind, "bf16", 16)
