@@ -20,6 +20,7 @@
 #include "gemv_tma.cuh"
 #include "gemv_flat_tma.cuh"
 #include "gemv_rowblk.cuh"
+#include "serve_common.h"
 
 namespace chpe {
 
@@ -1908,6 +1909,7 @@ void Engine::generate_processed(const uint32_t* prompt, size_t n_prompt, size_t 
   if (!(repetition > 0.f) || !std::isfinite(repetition) || !std::isfinite(frequency) || !std::isfinite(presence))
     throw std::runtime_error("penalties must be finite and repetition above 0");
   if (n_bias > 65535) throw std::runtime_error("at most 65535 biases");
+  const DeviceScope scope(device_);  // the buffer and the kernels below go to the engine's device, whatever the caller's is
   forward(prompt, n_prompt, 0);
   if (n_gen == 0) return;
   kv_ensure(n_prompt + n_gen);

@@ -1,0 +1,65 @@
+"""chpe_generate_processed after prompts that go through the single-token step, the
+batched step or both, and with another device current."""
+import threading
+from contextlib import closing
+
+import numpy as np
+import pytest
+
+import chpe_qwen_engine_b200 as chpe
+from _ops_ref import logits
+from _util import archive
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+WORDS = np.array([11, 2222, 33333, 11, 2222, 151000, 7, 11, 2222, 5, 5, 90000, 7, 11, 42, 2222, 11], np.uint32)
+RULES = dict(repetition=1.3, frequency=0.25, presence=0.5, bias={500: 1.5, 2222: -2.0})
+
+
+def engine(device=0):
+    return chpe.Engine.from_bytes(archive(chpe.SYNTH_3B_W4), chpe.SYNTH_ARCH[chpe.SYNTH_3B_W4], 64, device=device)
+
+
+def on_host(e, prompt, n_gen):
+    """The rules in f32, one rounding each, on every step's logits."""
+    e.forward_tokens(prompt)
+    said, ids, vals = [int(t) for t in prompt], np.array([list(RULES["bias"])]), np.float32([list(RULES["bias"].values())])
+    for i in range(n_gen):
+        if i:
+            e.forward_decode(said[-1], len(said) - 1)
+        _, t = logits(e.logits()[None], np.array([said]), [len(prompt)], None, np.float32([1.3]), np.float32([0.25]), np.float32([0.5]),
+                      ids, vals, kind=np.float32)
+        said.append(int(t[0]))
+    return said[len(prompt):]
+
+
+@pytest.mark.parametrize("n", [1, 3, 7, 8, 9, 16, 17])
+def test_prompts_of_every_path(n):
+    with closing(engine()) as e:
+        first = e.generate_processed(WORDS[:n], 10, **RULES).tolist()  # the engine's first call
+        assert first == on_host(e, WORDS[:n], 10)
+        assert e.generate_processed(WORDS[:n], 10, **RULES).tolist() == first
+        assert np.array_equal(e.generate_processed(WORDS[:n], 10), e.generate(WORDS[:n], 10))
+
+
+def test_called_from_another_thread():
+    with closing(engine()) as e:
+        want = e.generate_processed(WORDS[:3], 6, **RULES).tolist()
+        got = []
+        t = threading.Thread(target=lambda: got.extend(e.generate_processed(WORDS[:3], 6, **RULES).tolist()))
+        t.start()
+        t.join()
+        assert got == want
+
+
+@pytest.mark.skipif(torch is None or torch.cuda.device_count() < 2, reason="needs two GPUs")
+@pytest.mark.parametrize("device", [0, 1])
+def test_with_another_device_current(device):
+    """Prompts below 8 tokens do not pass the batched step, which makes the engine's device current."""
+    with closing(engine(device)) as e:
+        want = e.generate_processed(WORDS[:3], 6, **RULES).tolist()
+        with torch.cuda.device(1 - device):
+            torch.zeros(1, device=f"cuda:{1 - device}")
+            assert e.generate_processed(WORDS[:3], 6, **RULES).tolist() == want
+            assert torch.cuda.current_device() == 1 - device
