@@ -1766,6 +1766,11 @@ void Engine::kv_load(uint32_t layer, uint32_t pos0, uint32_t n, const float* k, 
   }
 }
 
+// `used` and `more` positions fit (a caller's size_t may make their sum wrap).
+static void check_room(uint64_t used, uint64_t more, uint64_t max_seq) {
+  if (used > max_seq || more > max_seq - used) throw std::runtime_error("sequence exceeds max_seq_len");
+}
+
 void Engine::run_steps(size_t n) {
   for (size_t i = 0; i < n; i++) CK(cudaGraphLaunch(graph_, stream_));
 }
@@ -1804,7 +1809,7 @@ void Engine::debug_wait_timeout(uint32_t polls) {
 void Engine::forward(const uint32_t* toks, size_t n, uint32_t start_pos) {
   if (n == 0) return;
   if (ops_->empty()) throw std::runtime_error("tensor parallel engine: call tp_connect first");
-  if ((uint64_t)start_pos + n > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
+  check_room(start_pos, n, max_seq_);
   if (start_pos == 0) kv_reset();  // a new sequence
   kv_ensure((uint64_t)start_pos + n);
   if (!graph_) {
@@ -1853,7 +1858,7 @@ void Engine::forward(const uint32_t* toks, size_t n, uint32_t start_pos) {
   h_st_->done_ctas = 0;
   h_st_->n_gen = 0;
   CK(cudaMemcpyAsync(d_st_, h_st_, sizeof(StepState), cudaMemcpyHostToDevice, stream_));
-  if (n + 1 > h_tok_cap_) throw std::runtime_error("token buffer too small");
+  if (n >= h_tok_cap_) throw std::runtime_error("token buffer too small");
   for (size_t i = 0; i < n; i++) {
     h_tok_[i] = toks[i];
     if (i > 0)
@@ -1867,7 +1872,7 @@ void Engine::forward(const uint32_t* toks, size_t n, uint32_t start_pos) {
 
 void Engine::generate(const uint32_t* prompt, size_t n_prompt, size_t n_gen, uint32_t* out_tokens) {
   if (n_prompt == 0) throw std::runtime_error("empty prompt");
-  if (n_prompt + n_gen > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
+  check_room(n_prompt, n_gen, max_seq_);
   forward(prompt, n_prompt, 0);
   if (n_gen == 0) return;
   kv_ensure(n_prompt + n_gen);
@@ -1904,7 +1909,7 @@ void Engine::generate_processed(const uint32_t* prompt, size_t n_prompt, size_t 
                                 const float* bias_values, size_t n_bias, const uint32_t* mask,
                                 uint32_t* out_tokens) {
   if (n_prompt == 0) throw std::runtime_error("empty prompt");
-  if (n_prompt + n_gen > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
+  check_room(n_prompt, n_gen, max_seq_);
   if (tp_world_ > 1) throw std::runtime_error("generate_processed runs on one GPU");
   if (!(repetition > 0.f) || !std::isfinite(repetition) || !std::isfinite(frequency) || !std::isfinite(presence))
     throw std::runtime_error("penalties must be finite and repetition above 0");
@@ -1977,8 +1982,8 @@ void Engine::verify(const uint32_t* toks, size_t m, uint32_t pos, float* logits_
     last_verify_batched_ = 1;
     return;
   }
-  if ((uint64_t)pos + m > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
-  if (m + 1 > h_tok_cap_) throw std::runtime_error("too many candidates");
+  check_room(pos, m, max_seq_);
+  if (m >= h_tok_cap_) throw std::runtime_error("too many candidates");
   if (pos == 0) kv_reset();
   kv_ensure((uint64_t)pos + m);
   if (!graph_) {
@@ -2044,8 +2049,8 @@ static size_t lookup_draft(const std::vector<uint32_t>& h, uint32_t ngram, size_
 void Engine::speculative_generate(const uint32_t* prompt, size_t n_prompt, size_t n_gen, uint32_t draft,
                                   uint32_t ngram, uint32_t* out, uint64_t* stats) {
   if (n_prompt == 0) throw std::runtime_error("empty prompt");
-  if (n_prompt + n_gen > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
-  if (draft + 1 > h_tok_cap_) throw std::runtime_error("draft longer than the token buffer");
+  check_room(n_prompt, n_gen, max_seq_);
+  if (draft >= h_tok_cap_) throw std::runtime_error("draft longer than the token buffer");
   uint64_t rounds = 0, proposed = 0, accepted = 0;
   forward(prompt, n_prompt, 0);
   if (n_gen == 0) return;
@@ -2088,7 +2093,7 @@ void Engine::speculative_generate(const uint32_t* prompt, size_t n_prompt, size_
 
 float Engine::timed_greedy_steps(size_t n) {
   if (!graph_) throw std::runtime_error("run forward() first");
-  if ((uint64_t)pos_ + n > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
+  check_room(pos_, n, max_seq_);
   kv_ensure((uint64_t)pos_ + n);
   int32_t one = 1, zero = 0;
   CK(cudaMemcpyAsync(&d_st_->feed_argmax, &one, 4, cudaMemcpyHostToDevice, stream_));
@@ -2115,7 +2120,7 @@ float Engine::timed_greedy_steps(size_t n) {
 
 double Engine::timed_host_steps(const uint32_t* toks, size_t n, float* logits_host) {
   if (!graph_) throw std::runtime_error("run forward() first");
-  if ((uint64_t)pos_ + n > max_seq_) throw std::runtime_error("sequence exceeds max_seq_len");
+  check_room(pos_, n, max_seq_);
   kv_ensure((uint64_t)pos_ + n);
   CK(cudaStreamSynchronize(stream_));
   uint64_t t0 = now_ns();

@@ -1,5 +1,6 @@
 """chpe_generate_processed after prompts that go through the single-token step, the
 batched step or both, and with another device current."""
+import ctypes as C
 import threading
 from contextlib import closing
 
@@ -63,3 +64,21 @@ def test_with_another_device_current(device):
             torch.zeros(1, device=f"cuda:{1 - device}")
             assert e.generate_processed(WORDS[:3], 6, **RULES).tolist() == want
             assert torch.cuda.current_device() == 1 - device
+
+
+@pytest.mark.parametrize("n_gen", [-1, -3, 2 ** 64 - 3, 2 ** 63, 62])
+def test_lengths_whose_sum_wraps_are_refused(n_gen):
+    """A negative number of tokens arrives as a size_t near 2^64."""
+    u32 = lambda a: a.ctypes.data_as(C.POINTER(C.c_uint32))  # noqa: E731
+    out = np.full(64, 7, np.uint32)
+    with closing(engine()) as e:
+        e.generate(WORDS[:3], 2)
+        n, L = C.c_size_t(n_gen), chpe.lib()
+        assert L.chpe_generate_processed(e.ctx, u32(WORDS), 3, n, 1.0, 0.0, 0.0, None, None, 0, None, u32(out)) == -1
+        assert L.chpe_generate(e.ctx, u32(WORDS), 3, n, u32(out)) == -1
+        assert L.chpe_speculative_generate(e.ctx, u32(WORDS), 3, n, 4, 3, u32(out), None) == -1
+        assert "max_seq_len" in L.chpe_last_error(e.ctx).decode()
+        assert L.chpe_speculative_generate(e.ctx, u32(WORDS), 3, 4, 2 ** 32 - 1, 3, u32(out), None) == -1
+        assert L.chpe_bench_greedy(e.ctx, n, C.byref(C.c_float())) == -1
+        assert (out == 7).all()
+        assert e.generate_processed(WORDS[:3], 61).size == 61  # to the last position
