@@ -1893,15 +1893,17 @@ void Engine::generate(const uint32_t* prompt, size_t n_prompt, size_t n_gen, uin
 
 // Takes the token that the rules chose: into the history (whose length grows by
 // one), the list of generated tokens and the step's result, which feeds it to the
-// next step.  -1, no token left, is kept in the list and fed as 0.
-static __global__ void commit_token_kernel(const int32_t* chosen, int32_t* history, int32_t* length,
-                                           int32_t* generated, StepResult* res) {
+// next step, with its logit as the model gave it.  -1, no token left, is kept in the list
+// and fed as 0.
+static __global__ void commit_token_kernel(const int32_t* chosen, const float* logits, int32_t* history,
+                                           int32_t* length, int32_t* generated, StepResult* res) {
   if (threadIdx.x != 0) return;
   const int32_t t = *chosen;
   history[*length] = t;
   *length += 1;
   *generated = t;
   res->argmax_token = t < 0 ? 0u : (uint32_t)t;
+  res->max_logit = t < 0 ? -1e30f : logits[t];
 }
 
 void Engine::generate_processed(const uint32_t* prompt, size_t n_prompt, size_t n_gen, float repetition,
@@ -1963,7 +1965,7 @@ void Engine::generate_processed(const uint32_t* prompt, size_t n_prompt, size_t 
         presence != 0.f ? d_pen + 2 : nullptr, n_bias ? d_ids : nullptr, n_bias ? d_vals : nullptr, 0,
         (uint32_t)n_bias, d_mask, 0, nullptr, 0, d_len + 2, stream_);
     if (rc != 0) throw std::runtime_error(chpe_last_error(nullptr));
-    commit_token_kernel<<<1, 32, 0, stream_>>>(d_len + 2, d_hist, d_len, d_out + i, d_res_);
+    commit_token_kernel<<<1, 32, 0, stream_>>>(d_len + 2, d_logits_, d_hist, d_len, d_out + i, d_res_);
     CK(cudaGetLastError());
   }
   CK(cudaMemcpyAsync(out_tokens, d_out, n_gen * 4, cudaMemcpyDeviceToHost, stream_));

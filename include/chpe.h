@@ -187,7 +187,8 @@ int chpe_generate(void *ctx, const uint32_t *prompt, size_t n_prompt, size_t n_g
  * biases (host arrays; of several for one token the last counts), and a mask of
  * ceil(vocab/32) host words that holds for every step (NULL: none).  With no
  * rule it gives chpe_generate's tokens.  chpe_get_last_logits gives the last
- * step's logits as the model gave them.  One GPU.  0 on success; -1 on error, among
+ * step's logits as the model gave them, chpe_get_last_argmax the last chosen
+ * token and chpe_get_last_max_logit that token's logit among them.  One GPU.  0 on success; -1 on error, among
  * them penalties that are not finite, a repetition of 0 or less, and a step that
  * is left without a token (out_tokens holds 0xFFFFFFFF there). */
 int chpe_generate_processed(void *ctx, const uint32_t *prompt, size_t n_prompt, size_t n_gen,

@@ -82,3 +82,19 @@ def test_lengths_whose_sum_wraps_are_refused(n_gen):
         assert L.chpe_bench_greedy(e.ctx, n, C.byref(C.c_float())) == -1
         assert (out == 7).all()
         assert e.generate_processed(WORDS[:3], 61).size == 61  # to the last position
+
+
+def test_the_last_result_is_of_the_chosen_token():
+    with closing(engine()) as e:
+        for n in (3, 8):  # the last prompt token by the single-token step, by the batched one
+            for n_gen in (1, 2, 7):
+                got = e.generate_processed(WORDS[:n], n_gen, **RULES)
+                r = e.last_result()
+                assert r.argmax_token == got[-1] and r.max_logit == e.logits()[got[-1]]
+            mask = np.zeros((e.vocab + 31) // 32, np.uint32)
+            mask[777 // 32] = 1 << (777 % 32)
+            e.generate_processed(WORDS[:n], 3, mask=mask)
+            r, x = e.last_result(), e.logits()
+            assert r.argmax_token == 777 and r.max_logit == x[777] < x.max()
+            e.generate_processed(WORDS[:n], 3)
+            assert e.last_result().max_logit == e.logits().max()
