@@ -391,8 +391,13 @@ int chpe_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, in
  * a page outside 0..num_pages-1 are left out.  Nothing beyond a sequence's
  * length is used, whatever the pages hold there.  lse [batch][num_heads] float
  * (or NULL): the natural logarithm of the softmax's sum.
- * A query, key or value in use that is not finite makes the outputs it enters
- * NaN or infinite.
+ * What is not finite: a score of -inf (an infinite key against queries of the
+ * cache's type) has weight 0, and where every score is -inf, out = 0 and
+ * lse = -inf as for no entry.  A score of +inf or NaN makes its query head's out
+ * and lse NaN, and so does an infinite key under float queries, which enter in
+ * parts (unless no part is 0 and all have one sign).  A value that is infinite or
+ * NaN makes its dimension infinite or NaN for the query heads of its kv head, at
+ * weight 0 too; lse is not touched.
  * The cache has q's type, or any when q is float.  Results do not depend on
  * timing: the same call gives the same bits.
  * workspace: chpe_attention_decode_paged_workspace(head_dim) bytes (0 for an

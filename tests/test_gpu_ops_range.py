@@ -3,6 +3,7 @@ as in test_gpu_ops.py."""
 import numpy as np
 import pytest
 
+from _ops_ref import attention
 from test_gpu_ops import DEV, check_paged, close, f64, i32, paged_case, put
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +89,77 @@ def test_paged_attention_large_bf16_values(kind, lens, H, KV, D):
     q, tk, tv, table, xq, xk, xv = paged_case(rng, kind, "bf16", lens, H, KV, D, 16)
     tv = tv * 2.0 ** 112
     check_paged(q, tk, tv, table, lens, xq, xk, f64(tv), kind, "bf16", 16)
+
+
+# ---- what is not finite ----------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n, B", [(40, 1), (3000, 1), (3000, 70)])  # in one CTA, cut into many and into few records
+@pytest.mark.parametrize("H, KV, D", [(4, 2, 64), (8, 8, 128), (4, 1, 256)])
+def test_paged_attention_infinite_scores(kind, n, B, H, KV, D):
+    inf = float("inf")
+    rng = np.random.default_rng(4)
+    G = H // KV
+    page, each = 64, -(-n // 64)
+    tk, _ = put(rng.standard_normal((each, page, KV, D)), kind)
+    tv, _ = put(rng.standard_normal((each, page, KV, D)), kind)
+    q, _ = put(np.abs(rng.standard_normal((B, H, D))) + 0.1, kind)  # the sign of a key's infinity is its score's
+    table = i32(np.arange(each)[None]).expand(B, -1)
+    lens = i32([n] * B)
+    lse = torch.empty(B, H, device=DEV)
+
+    def call(k, v=tv, qq=q):
+        return ops.attention_decode_paged(qq, k, v, table, lens, lse=lse).clone(), lse.clone()
+    clean, clean_lse = call(tk)
+    others = torch.arange(H, device=DEV) >= G
+    at = n - 5
+    for value, kind_of in ((float("nan"), "nan"), (inf, "nan"), (-inf, "gone")):
+        k = tk.clone()
+        k[at // page, at % page, 0, 3] = value  # kv head 0
+        out, l = call(k)
+        assert torch.equal(out[:, others], clean[:, others]) and torch.equal(l[:, others], clean_lse[:, others])
+        if kind_of == "nan":
+            assert torch.isnan(out[:, :G]).all() and torch.isnan(l[:, :G]).all()
+        else:  # weight 0: as if the position were not there
+            keep = np.arange(n) != at
+            kk, vv = (f64(t).reshape(-1, KV, D)[:n][keep] for t in (tk, tv))
+            pad = np.zeros((each * page - n + 1, KV, D))
+            for b in (0, B - 1):
+                ref, rl, bo, bl = attention(f64(q)[b:b + 1], np.concatenate((kk, pad)).reshape(each, page, KV, D),
+                                            np.concatenate((vv, pad)).reshape(each, page, KV, D), np.arange(each)[None], [n - 1],
+                                            D ** -0.5, page, kind, kind)
+                close(out[b:b + 1, :G], ref[:, :G], bo[:, :G], kind)
+                assert np.all(np.abs(f64(l)[b, :G] - rl[0, :G]) <= bl[0, :G])
+    k = tk.clone()
+    k[:, :, 0, 3] = -inf  # every score of kv head 0
+    out, l = call(k)
+    assert not out[:, :G].any() and torch.isneginf(l[:, :G]).all()
+    assert torch.equal(out[:, others], clean[:, others])
+    k[0, :, 0, 3] = 1.0  # all but the first page's
+    out, l = call(k)
+    assert torch.isfinite(out).all() and torch.isfinite(l).all()
+    v = tv.clone()
+    v[at // page, at % page, 0, 9] = inf
+    out, l = call(tk, v)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[:, :G, 9] = True
+    assert torch.equal(~torch.isfinite(out), bad) and torch.equal(out[~bad], clean[~bad]) and torch.equal(l, clean_lse)
+    qq = q.clone()
+    qq[0, 0, 3] = inf
+    out, l = call(tk, tv, qq)
+    assert torch.isnan(out[0, 0]).all() and torch.isnan(l[0, 0])
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, 0] = True
+    assert torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_paged_attention_infinite_keys_under_float_queries(cache):
+    """The parts of a float query meet an infinite key one by one: 0 times infinity among them."""
+    tk = torch.zeros(1, 16, 1, 64, device=DEV, dtype=torch.float16 if cache == "f16" else torch.bfloat16)
+    tv = torch.ones_like(tk)
+    tk[0, 2, 0, 0] = -float("inf")
+    q = torch.ones(1, 1, 64, device=DEV)
+    lse = torch.zeros(1, 1, device=DEV)
+    out = ops.attention_decode_paged(q, tk, tv, i32([[0]]), i32([5]), lse=lse)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    assert torch.equal(ops.attention_decode_paged(q, tk, tv, i32([[0]]), i32([2])), torch.ones_like(q))
