@@ -38,7 +38,7 @@ ENGINE_SRCS = ["engine.cu", "engine_verify.cu", "attention_noalloc.cu", "deltane
                "chpe_c_api.cpp", "chpe_maps.c"]
 ENGINE_DEPS = ENGINE_SRCS + ["engine.h", "engine_types.h", "gemv.cuh", "attention.cuh",
                              "aux_kernels.cuh", "gemv_tma.cuh", "gemv_flat_tma.cuh", "gemv_rowblk.cuh", "device_common.cuh", "chpe_maps.h",
-                             "tc_common.cuh", "bgemm_tc.cuh", "serve_common.h",
+                             "tc_common.cuh", "bgemm_tc.cuh", "serve_common.h", "buffer_rows.h",
                              "qwen3b_cell_map.inc", "../../include/chpe.h"]
 SYNTH_SRCS = ["chpe_synth.c", "chpe_maps.c"]
 SYNTH_DEPS = SYNTH_SRCS + ["chpe_synth.h", "chpe_maps.h", "qwen3b_cell_map.inc"]

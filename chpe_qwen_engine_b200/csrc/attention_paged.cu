@@ -887,6 +887,21 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
     c.ptr(page_table, "page_table", 4);
   }
   if (c.rc) return c.done();
+  {
+    using chpe::Rows;
+    const int64_t n = batch, b = (int64_t)es;
+    const uint64_t rows = num_pages && max_pages ? (uint64_t)num_pages * page_size : 0, row = 2ull * num_kv_heads * head_dim;
+    const Rows in[] = {{"q", q, least * b, n, q_stride, b}, chpe::pool("k_cache", k_cache, rows, row),
+                       chpe::pool("v_cache", v_cache, rows, row),
+                       {"page_table", rows ? page_table : nullptr, 4ll * max_pages, n, table_stride, 4}, {"seq_lens", seq_lens, 4 * n}};
+    const Rows to[] = {{"out", out, least * b, n, out_stride, b}, {"lse", lse, 4 * n * num_heads},
+                        {"workspace", workspace, (int64_t)chpe_attention_decode_paged_workspace(head_dim)}};
+    for (int o = 0; o < 3; o++) {
+      for (const Rows& i : in) c.apart(to[o], i);
+      for (int i = 0; i < o; i++) c.apart(to[o], to[i]);
+    }
+    if (c.rc) return c.done();
+  }
 
   PagedLaunch P{};
   P.q = q, P.q_stride = q_stride;

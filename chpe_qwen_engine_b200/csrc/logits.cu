@@ -467,6 +467,25 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
   c.ptr_or_null(out, "out", 4);
   c.ptr_or_null(argmax, "argmax", 4);
   if (c.rc) return c.done();
+  const bool in_place = dtype == CHPE_F32 && out == logits && (batch == 1 || out_stride == logits_stride);
+  {
+    using chpe::Rows;
+    const int64_t n = batch, v = vocab;
+    const Rows in[] = {{"history", history, 4ll * history_len, n, history_stride, 4},
+                       {"logits", logits, v * (int64_t)es, n, logits_stride, (int64_t)es},
+                       {"bias_ids", bias_ids, 4ll * max_bias, n, bias_stride, 4}, {"bias_values", bias_values, 4ll * max_bias, n, bias_stride, 4},
+                       {"mask", mask, 4 * words, n, mask_stride, 4}, {"prompt_lens", prompt_lens, 4 * n},
+                       {"total_lens", total_lens, 4 * n}, {"repetition", repetition, 4 * n},
+                       {"frequency", frequency, 4 * n}, {"presence", presence, 4 * n}};
+    const Rows x("out", out, 4 * v, n, out_stride, 4), t("argmax", argmax, 4 * n);
+    for (int i = 0; i < 10; i++) {
+      if (!(i == 1 && in_place)) c.apart(x, in[i]);
+      // (one row's token may go behind its history: it is written when all has been read)
+      if (!(i == 0 && n == 1)) c.apart(t, in[i]);
+    }
+    c.apart(x, t);
+    if (c.rc) return c.done();
+  }
 
   LogitsLaunch P{};
   P.logits = logits, P.stride = logits_stride, P.vocab = vocab;
@@ -483,7 +502,7 @@ extern "C" int chpe_logits_process(const void* logits, int dtype, int64_t logits
   if (max_bias) P.bias_ids = bias_ids, P.bias_values = bias_values, P.bias_stride = bias_stride, P.max_bias = max_bias;
   P.mask = mask, P.mask_stride = mask_stride;
   P.out = out, P.out_stride = out_stride, P.argmax = argmax;
-  P.in_place = dtype == CHPE_F32 && out == logits && (batch == 1 || out_stride == logits_stride);
+  P.in_place = in_place;
   const bool vec = reinterpret_cast<uintptr_t>(logits) % (4 * es) == 0 && (batch == 1 || logits_stride % 4 == 0) &&
                    (!out || (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (batch == 1 || out_stride % 4 == 0)));
   chpe::DeviceScope scope(c.launch_device());

@@ -343,6 +343,22 @@ extern "C" int chpe_qk_norm_rope(const void* q, const void* k, const void* v, in
   c.ptr_or_null(q_weight, "q_weight", 16);
   c.ptr_or_null(k_weight, "k_weight", 16);
   if (c.rc) return c.done();
+  {
+    // q_out may be q and k_out k, row by row; else what is written meets nothing
+    using chpe::Rows;
+    const int64_t n = num_tokens, b = (int64_t)es, w = head_dim * (int64_t)sizeof(float);
+    const Rows in[] = {{"q", q, hq * b, n, q_stride, b}, {"k", k, hk * b, n, k_stride, b},
+                       {"v", k_cache ? v : nullptr, hk * b, n, v_stride, b}, {"q_weight", q_weight, w}, {"k_weight", k_weight, w},
+                       {"positions", rope_dim ? positions : nullptr, 4 * n}, {"slots", k_cache ? slots : nullptr, 8 * n}};
+    const Rows out[] = {{"q_out", q_out, hq * b, n, q_out_stride, b}, {"k_out", k_out, hk * b, n, k_out_stride, b},
+                        chpe::pool("k_cache", k_cache, cache_rows, hk * 2), chpe::pool("v_cache", v_cache, cache_rows, hk * 2)};
+    for (int o = 0; o < 4; o++) {
+      for (int i = 0; i < 7; i++)
+        if (!(o == i && out[o].p == in[i].p && (n == 1 || out[o].stride == in[i].stride) && o < 2)) c.apart(out[o], in[i]);
+      for (int i = 0; i < o; i++) c.apart(out[o], out[i]);
+    }
+    if (c.rc) return c.done();
+  }
 
   P.q = q, P.k = k, P.v = v;
   P.q_stride = q_stride, P.k_stride = k_stride, P.v_stride = v_stride;

@@ -6,6 +6,8 @@
 // address, a freed one, or one on another GPU is answered with -1 instead of a
 // fault on the device.  The launch goes to the device that holds the buffers,
 // which need not be the current one; the current device is left as it was.
+// Buffers that the call writes must not overlap the others, but for what an entry
+// point allows.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -14,6 +16,7 @@
 #include <string>
 
 #include "../../include/chpe.h"
+#include "buffer_rows.h"
 #include "engine.h"
 
 namespace chpe {
@@ -67,6 +70,13 @@ struct ServeCall {
   }
   void ptr_or_null(const void* p, const char* what, uintptr_t align) {
     if (p) ptr(p, what, align);
+  }
+  // out: rows that the call writes; other: rows that it reads, or writes too.  For checked
+  // pointers, behind the checks of strides.
+  void apart(const Rows& out, const Rows& other) {
+    if (rc || !out.meets(other)) return;
+    snprintf(msg, sizeof(msg), "%s overlaps %s", out.name, other.name);
+    rc = -1;
   }
   // The device to launch on: that of the buffers, or the current one for managed memory.
   int launch_device() {

@@ -342,8 +342,10 @@ int chpe_attention_decode_noalloc(const float *q, const float *k, const float *v
  * captured into a graph.  The buffers lie on one device, which need not be
  * the current one.  They keep no state between calls, and calls on different
  * streams may overlap (attention: with a workspace each).
+ * What a call writes shares no byte with what it reads or writes beside it, except
+ * where an operator says so; rows that lie side by side in one buffer share none.
  * Return value: 0; -1 for an argument they refuse (NULL, misaligned or host
- * pointers, sizes and types outside the limits), -2 for too small a workspace,
+ * pointers, sizes and types outside the limits, overlaps), -2 for too small a workspace,
  * -3 for a CUDA error at the launch (the outputs are undefined then);
  * chpe_last_error(NULL) says why. */
 #define CHPE_F32 0
@@ -365,8 +367,7 @@ int chpe_attention_decode_noalloc(const float *q, const float *k, const float *v
  * NULL) the keys, in q's type; k_cache and v_cache (both or neither) row
  * slots[t] of each token's k and v.  A slot outside 0..cache_rows-1 (a padded
  * token's -1) stores nothing.  Two tokens of a call must not share a row.
- * q_out may be q itself with q's stride, k_out k itself; otherwise outputs
- * must not overlap inputs.  Without a cache, v, v_cache, slots may be NULL and
+ * q_out may be q itself with q's stride, k_out k itself.  Without a cache, v, v_cache, slots may be NULL and
  * k_out is needed.  The cache has the type of q, k and v, or any when those
  * are float.  Buffers and strides are multiples of 16 bytes. */
 int chpe_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, int64_t q_stride,
@@ -383,7 +384,7 @@ int chpe_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, in
  * t < seq_lens[b] (the new token's own among them: append it first), query
  * heads h*G .. h*G+G-1 on kv head h, G = num_heads / num_kv_heads of any size.
  * q and out [batch][num_heads][head_dim] of dtype, rows q_stride / out_stride
- * apart (multiples of 16 bytes); out must not overlap q or the cache.
+ * apart (multiples of 16 bytes).
  * page_table: rows of max_pages entries, table_stride apart (0: one row for all);
  * entry p of a row is the page of positions p*page_size ..; page_size a power of
  * two from 16 to 65536.  Sequences may share pages.  seq_lens [batch] int32; a
@@ -430,7 +431,8 @@ int chpe_attention_decode_paged(const void *q, int dtype, int64_t q_stride, cons
  * out [batch][out_stride] float gets every x (NULL: not wanted) and may be the
  * logits themselves where those are float with the same stride; argmax [batch]
  * (NULL: not wanted) the lowest token of the largest x: NaN never wins, and -1
- * means that no x is above -inf.  Each step is rounded to f32 by itself. */
+ * means that no x is above -inf.  One row's argmax may lie in its own history behind
+ * the total length.  Each step is rounded to f32 by itself. */
 int chpe_logits_process(const void *logits, int dtype, int64_t logits_stride, uint32_t batch,
                         uint32_t vocab, const int32_t *history, int64_t history_stride,
                         uint32_t history_len, const int32_t *prompt_lens, const int32_t *total_lens,

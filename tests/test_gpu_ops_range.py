@@ -3,6 +3,7 @@ as in test_gpu_ops.py."""
 import numpy as np
 import pytest
 
+import chpe_qwen_engine_b200 as chpe
 from _ops_ref import attention
 from test_gpu_ops import DEV, check_paged, close, f64, i32, paged_case, put
 
@@ -163,3 +164,90 @@ def test_paged_attention_infinite_keys_under_float_queries(cache):
     out = ops.attention_decode_paged(q, tk, tv, i32([[0]]), i32([5]), lse=lse)
     assert torch.isnan(out).all() and torch.isnan(lse).all()
     assert torch.equal(ops.attention_decode_paged(q, tk, tv, i32([[0]]), i32([2])), torch.ones_like(q))
+
+
+# ---- buffers that overlap ------------------------------------------------------------
+def refused(what, f, *a, **kw):
+    with pytest.raises(chpe.ChpeError, match=what):
+        f(*a, **kw)
+
+
+def test_qk_refuses_overlaps():
+    T, H, KV, D = 5, 4, 2, 64
+    wide = torch.randn(T, (H + 2 * KV) * D + 2 * D, device=DEV).half()
+    part = lambda first, heads: wide[:, first * D:(first + heads) * D].unflatten(1, (heads, D))  # noqa: E731
+    q, k, v = part(0, H), part(H, KV), part(H + KV, KV)
+    freq, pos = ops.rope_inv_freq(1e4, D), i32(range(T))
+    kc, vc = torch.zeros(2, 2, 16, KV, D, device=DEV, dtype=torch.float16)
+    slots = torch.arange(T, device=DEV)
+    a = (q, k, v, pos, freq)
+    cache = dict(k_cache=kc, v_cache=vc, slots=slots)
+    want = [t.clone() for t in ops.qk_norm_rope(*a)]
+    before = wide.clone()
+    refused("q_out overlaps k", ops.qk_norm_rope, *a, q_out=part(H, H))
+    refused("q_out overlaps q", ops.qk_norm_rope, *a, q_out=part(1, H))
+    refused("q_out overlaps v", ops.qk_norm_rope, *a, q_out=part(H + KV, H), **cache)
+    both = torch.zeros(T, (H + KV) * D, device=DEV, dtype=torch.float16)
+    refused("k_out overlaps q_out", ops.qk_norm_rope, *a, q_out=both[:, :H * D].unflatten(1, (H, D)),
+            k_out=both[:, (H - 1) * D:(H + 1) * D].unflatten(1, (KV, D)))
+    refused("k_cache overlaps q", ops.qk_norm_rope, q, k, v, pos, freq, k_cache=wide.view(-1)[:16 * KV * D].view(1, 16, KV, D),
+            v_cache=vc[:1], slots=slots)
+    refused("v_cache overlaps k_cache", ops.qk_norm_rope, *a, k_cache=kc, v_cache=kc, slots=slots)
+    rows = torch.zeros(T, 2, KV, D, device=DEV, dtype=torch.float16)
+    refused("q_out overlaps positions", ops.qk_norm_rope, rows[:, 0].contiguous(), rows[:, 0].contiguous(), None, rows.view(-1).view(torch.int32)[:T],
+            freq, q_out=rows.view(-1)[:T * KV * D].view(T, KV, D))
+    torch.cuda.synchronize()
+    assert torch.equal(wide, before) and not kc.any()
+    # side by side in one buffer they share nothing, and in place is allowed
+    out, _ = ops.qk_norm_rope(*a, q_out=q, k_out=k, **cache)
+    assert torch.equal(out, want[0]) and torch.equal(k, want[1]) and torch.equal(wide[:, (H + KV) * D:], before[:, (H + KV) * D:])
+    wide.copy_(before)
+    tail = wide[:, -2 * D:].unflatten(1, (KV, D))  # behind v in the same rows
+    assert torch.equal(ops.qk_norm_rope(*a, k_out=tail)[1], want[1])
+
+
+def test_attention_refuses_overlaps():
+    B, H, KV, D = 3, 4, 2, 64
+    g = torch.randn(B, 3 * H * D, device=DEV).half()
+    q = g[:, :H * D].unflatten(1, (H, D))
+    kc, vc = torch.randn(2, 4, 16, KV, D, device=DEV).half()
+    table, lens = i32([[0, 1], [2, 3], [1, 0]]), i32([20, 30, 1])
+    a = (q, kc, vc, table, lens)
+    want = ops.attention_decode_paged(*a)
+    refused("out overlaps q", ops.attention_decode_paged, *a, out=q)
+    refused("out overlaps q", ops.attention_decode_paged, *a, out=g[:, D:(H + 1) * D].unflatten(1, (H, D)))
+    refused("out overlaps k_cache", ops.attention_decode_paged, *a, out=kc.view(-1)[:B * H * D].view(B, H, D))
+    refused("out overlaps v_cache", ops.attention_decode_paged, *a, out=vc.view(-1)[-B * H * D:].view(B, H, D))
+    ws = ops.attention_workspace(D, DEV)
+    refused("lse overlaps seq_lens", ops.attention_decode_paged, *a[:4], ws[:12].view(torch.int32), lse=ws[:4 * B * H].view(torch.float32).view(B, H))
+    refused("workspace overlaps out", ops.attention_decode_paged, *a, out=ws[64:64 + 2 * B * H * D].view(torch.float16).view(B, H, D), workspace=ws)
+    refused("workspace overlaps page_table", ops.attention_decode_paged, q, kc, vc, ws[-24:].view(torch.int32).view(3, 2), lens, workspace=ws)
+    out = g[:, H * D:2 * H * D].unflatten(1, (H, D))  # behind the queries in the same rows
+    assert torch.equal(ops.attention_decode_paged(*a, out=out), want)
+    assert torch.equal(ops.attention_decode_paged(q, kc, kc, table, lens), ops.attention_decode_paged(q, kc, kc.clone(), table, lens))
+
+
+def test_logits_refuse_overlaps():
+    B, V = 3, 256
+    room = torch.randn(B, 3 * V, device=DEV)
+    x = room[:, :V]
+    want, am = ops.logits_process(x)
+    refused("out overlaps logits", ops.logits_process, x, out=room[:, 8:V + 8])
+    refused("out overlaps logits", ops.logits_process, x, out=room.view(-1)[:B * V].view(B, V))
+    half = torch.zeros(B, 2 * V, device=DEV, dtype=torch.float16)
+    refused("out overlaps logits", ops.logits_process, half[:, :V], out=half.view(torch.float32))
+    hist = torch.zeros(B, V, device=DEV, dtype=torch.int32)
+    refused("out overlaps history", ops.logits_process, x, history=hist, out=hist.view(torch.float32))
+    refused("out overlaps mask", ops.logits_process, x, mask=room.view(torch.int32)[:, V + 3:V + 11], out=room[:, V:2 * V])
+    few = torch.zeros(8, device=DEV, dtype=torch.int32)
+    refused("argmax overlaps total_lens", ops.logits_process, x, history=hist, total_lens=few[:B], argmax=few[1:B + 1])
+    refused("argmax overlaps history", ops.logits_process, x, history=hist, argmax=hist.view(-1)[:B])
+    refused("out overlaps argmax", ops.logits_process, x, out=room[:, V:2 * V], argmax=room.view(torch.int32)[0, V:V + B])
+    y, t = ops.logits_process(x, out=room[:, V:2 * V])
+    assert torch.equal(y, want) and torch.equal(t, am)
+    # one row's token behind the tokens so far
+    one, h = room[:1, :V], hist.view(-1)[:8].view(1, 8)
+    ops.logits_process(one, history=h, total_lens=i32([5]), argmax=h[0, 5:6], want_logits=False)
+    assert h[0, 5] == am[0] and not h[0, :5].any()
+    y, t = ops.logits_process(x, out=x)
+    assert torch.equal(room[:, :V], want) and torch.equal(t, am)
