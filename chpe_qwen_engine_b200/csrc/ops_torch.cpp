@@ -10,6 +10,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -87,7 +88,11 @@ struct Args {
       return nullptr;
     }
     if (!THPVariable_Check(at[i])) throw Misuse(std::string(name) + " must be a tensor");
-    return &THPVariable_Unpack(at[i]);
+    const Tensor& t = THPVariable_Unpack(at[i]);
+    // the operators have no gradient: one that autograd would expect must not get lost
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+      throw Unfit(std::string(name) + " requires a gradient, which this operator does not have: call it under torch.no_grad()");
+    return &t;
   }
   double number(int i, const char* name, double def) const {
     if (!at[i]) return def;

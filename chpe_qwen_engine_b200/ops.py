@@ -6,8 +6,9 @@ include/chpe.h states what each computes and what it refuses.  The functions
 (native, csrc/ops_torch.cpp) take shapes, strides and types from the tensors,
 check that they fit together, run on the current stream of the tensors' device
 (which need not be the current device), and raise ChpeError for what the
-library refuses and ValueError for tensors that do not fit.  Nothing is
-allocated when the outputs and the workspace are passed.  A cache is a pair of
+library refuses and ValueError for tensors that do not fit.  They have no
+gradients: where gradients are recorded, tensors that require one are refused.
+Nothing is allocated when the outputs and the workspace are passed.  A cache is a pair of
 contiguous tensors [num_pages, page_size, num_kv_heads, head_dim].
 """
 from __future__ import annotations

@@ -251,3 +251,26 @@ def test_logits_refuse_overlaps():
     assert h[0, 5] == am[0] and not h[0, :5].any()
     y, t = ops.logits_process(x, out=x)
     assert torch.equal(room[:, :V], want) and torch.equal(t, am)
+
+
+# ---- the torch layer ---------------------------------------------------------------------
+def test_gradients_are_refused_and_no_grad_is_not():
+    p = torch.nn.Parameter
+    q, kc = torch.randn(2, 2, 64, device=DEV).half(), torch.randn(2, 16, 2, 64, device=DEV).half()
+    pos, freq, w = i32([0, 1]), ops.rope_inv_freq(1e4, 64), p(torch.ones(64, device=DEV))
+    table, lens, x = i32([[0], [1]]), i32([3, 4]), torch.randn(2, 40, device=DEV)
+    one = torch.ones(2, device=DEV)
+    calls = [("q_weight", lambda: ops.qk_norm_rope(q, q, None, pos, freq, q_weight=w)),
+             ("k", lambda: ops.qk_norm_rope(q, p(q.clone()), None, pos, freq)),
+             ("q", lambda: ops.attention_decode_paged(p(q.clone()), kc, kc, table, lens)),
+             ("v_cache", lambda: ops.attention_decode_paged(q, kc, p(kc.clone()), table, lens)),
+             ("out", lambda: ops.attention_decode_paged(q, kc, kc, table, lens, out=p(q.clone()))),
+             ("logits", lambda: ops.logits_process(x.clone().requires_grad_() * 2)),
+             ("repetition", lambda: ops.logits_process(x, history=i32([[1], [2]]), repetition=p(one)))]
+    for name, call in calls:
+        with pytest.raises(ValueError, match=f"^{name} requires a gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
