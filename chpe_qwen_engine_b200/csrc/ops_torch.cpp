@@ -159,6 +159,12 @@ Tensor make(at::IntArrayRef shape, at::ScalarType type, int dev) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(at::Device(at::kCUDA, (c10::DeviceIndex)dev)));
 }
 
+// Autograd's record that t was written in place (as torch's own in-place operators leave it;
+// inference tensors have none).
+void written(const Tensor* t) {
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- errors ------------------------------------------------------------------------
 struct Refused {};  // the library's own message becomes ChpeError
 void check(int rc) {
@@ -284,6 +290,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject*
         u32(2 * f.n, "inv_freq"), qo->data_ptr(), qos, ko ? ko->data_ptr() : nullptr, kos,
         kc ? kc->data_ptr() : nullptr, kc ? vc->data_ptr() : nullptr, ct, (uint64_t)rows,
         kc ? vec<int64_t>(slots, "slots", at::kLong, T, dev) : nullptr, stream_of(dev)));
+    for (const Tensor* t : {qo, ko, kc, vc}) written(t);
     return pair(a.at[QO] ? again(a.at[QO]) : THPVariable_Wrap(q_made),
                 a.at[KO] ? again(a.at[KO]) : kc ? again(Py_None) : THPVariable_Wrap(k_made));
   });
@@ -325,6 +332,8 @@ PyObject* attention_decode_paged(PyObject*, PyObject* const* args, Py_ssize_t n,
         vec<int32_t>(&lens, "seq_lens", at::kInt, B, dev), u32(B, "the batch"), u32(H, "q"), u32(KVH, "the cache"),
         u32(D, "q"), (float)a.number(SCALE, "scale", 1.0 / std::sqrt((double)D)), out->data_ptr(), os,
         lse ? static_cast<float*>(lse->data_ptr()) : nullptr, ws->data_ptr(), (size_t)ws->numel(), stream_of(dev)));
+    written(out);
+    written(lse);
     return a.at[OUT] ? again(a.at[OUT]) : THPVariable_Wrap(made);
   });
 }
@@ -376,6 +385,8 @@ PyObject* logits_process(PyObject*, PyObject* const* args, Py_ssize_t n, PyObjec
         mask ? static_cast<const uint32_t*>(mask->data_ptr()) : nullptr, ms,
         out ? static_cast<float*>(out->data_ptr()) : nullptr, os, vec<int32_t>(am, "argmax", at::kInt, B, dev),
         stream_of(dev)));
+    written(out);
+    written(am);
     return pair(a.at[OUT] ? again(a.at[OUT]) : out ? THPVariable_Wrap(made) : again(Py_None),
                 a.at[ARGMAX] ? again(a.at[ARGMAX]) : THPVariable_Wrap(best));
   });

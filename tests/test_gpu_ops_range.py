@@ -274,3 +274,32 @@ def test_gradients_are_refused_and_no_grad_is_not():
             call()
         with torch.inference_mode():
             call()
+
+
+def test_what_is_written_counts_as_written():
+    """torch refuses a backward pass through values that an in-place write has replaced since."""
+    q, k = (torch.randn(2, 2, 64, device=DEV).half() for _ in range(2))
+    kc, vc = (torch.randn(2, 16, 2, 64, device=DEV).half() for _ in range(2))
+    lse, x = torch.zeros(2, 2, device=DEV), torch.randn(2, 40, device=DEV)
+    out, tok, base = torch.zeros_like(x), i32([0, 0]), torch.zeros(4, 2, 64, device=DEV).half()
+    at = lambda *ts: [t._version for t in ts]  # noqa: E731
+    v = at(q, k, kc, vc)
+    ops.qk_norm_rope(q, k, k, i32([0, 1]), None, q_out=base[:2], k_cache=kc, v_cache=vc, slots=torch.tensor([3, 17], device=DEV))
+    assert at(q, k, kc, vc) == [v[0], v[1], v[2] + 1, v[3] + 1] and base._version == 1
+    ops.qk_norm_rope(q, k, None, i32([0, 1]), None, q_out=q, k_out=k)
+    assert at(q, k) == [v[0] + 1, v[1] + 1]
+    v = at(q, kc, vc, lse, base)
+    ops.attention_decode_paged(q, kc, vc, i32([[0], [1]]), i32([3, 4]), out=base[2:], lse=lse)
+    assert at(q, kc, vc, lse, base) == [v[0], v[1], v[2], v[3] + 1, v[4] + 1]
+    v = at(x, out, tok)
+    ops.logits_process(x, out=out, argmax=tok)
+    assert at(x, out, tok) == [v[0], v[1] + 1, v[2] + 1]
+    w = torch.ones(2, 40, device=DEV, requires_grad=True)
+    y = (w * out).sum()  # needs `out` for w's gradient
+    ops.logits_process(x, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        held = torch.zeros_like(x)
+    ops.logits_process(x, out=held)
+    assert torch.equal(held, out)
