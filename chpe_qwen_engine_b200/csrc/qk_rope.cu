@@ -340,8 +340,8 @@ extern "C" int chpe_qk_norm_rope(const void* q, const void* k, const void* v, in
     c.ptr(slots, "slots", 8);
   }
   if (rope_dim) c.ptr(positions, "positions", 4);
-  c.ptr_or_null(q_weight, "q_weight", 16);
-  c.ptr_or_null(k_weight, "k_weight", 16);
+  c.ptr_or_null(q_weight, "q_weight", 4);  // (read value by value, once per warp)
+  c.ptr_or_null(k_weight, "k_weight", 4);
   if (c.rc) return c.done();
   {
     // q_out may be q and k_out k, row by row; else what is written meets nothing

@@ -369,7 +369,8 @@ int chpe_attention_decode_noalloc(const float *q, const float *k, const float *v
  * token's -1) stores nothing.  Two tokens of a call must not share a row.
  * q_out may be q itself with q's stride, k_out k itself.  Without a cache, v, v_cache, slots may be NULL and
  * k_out is needed.  The cache has the type of q, k and v, or any when those
- * are float.  Buffers and strides are multiples of 16 bytes. */
+ * are float.  q, k, v, the outputs, the caches and the strides are multiples of 16
+ * bytes; weights, positions and slots lie at multiples of their element. */
 int chpe_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, int64_t q_stride,
                       int64_t k_stride, int64_t v_stride, uint32_t num_tokens, uint32_t num_heads,
                       uint32_t num_kv_heads, uint32_t head_dim, const float *q_weight,

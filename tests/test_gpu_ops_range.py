@@ -303,3 +303,13 @@ def test_what_is_written_counts_as_written():
         held = torch.zeros_like(x)
     ops.logits_process(x, out=held)
     assert torch.equal(held, out)
+
+
+def test_norm_weights_at_any_float():
+    """A layer's weights out of one packed buffer."""
+    q, k = (torch.randn(3, 2, 64, device=DEV) for _ in range(2))
+    packed = torch.randn(1 + 64 + 2 + 64, device=DEV)
+    wq, wk = packed[1:65], packed[67:]
+    a = ops.qk_norm_rope(q, k, None, i32([0, 1, 2]), ops.rope_inv_freq(1e4, 64), q_weight=wq, k_weight=wk)
+    b = ops.qk_norm_rope(q, k, None, i32([0, 1, 2]), ops.rope_inv_freq(1e4, 64), q_weight=wq.clone(), k_weight=wk.clone())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
