@@ -3,7 +3,8 @@
 * libchpe.so        -- the product: C ABI + CUDA kernels for sm_100a (nvcc)
 * libchpe_synth.so  -- deterministic synthetic archive generator (gcc)
 * _ops.so           -- the batched decode operators on torch tensors, a CPython
-                       module over libchpe.so (g++, torch's headers)
+                       module over libchpe.so (g++, torch's headers; left out
+                       where torch is missing, rebuilt when torch changes)
 * chpe_fwd          -- the command-line front end over libchpe.so (the
                        reference's chpe_fwd contract)
 
@@ -11,6 +12,8 @@ Usage: python -m chpe_qwen_engine_b200.build [--force]
 """
 from __future__ import annotations
 
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -24,6 +27,7 @@ LIBCHPE = os.path.join(PKG, "libchpe.so")
 LIBSYNTH = os.path.join(PKG, "libchpe_synth.so")
 CHPE_FWD = os.path.join(PKG, "chpe_fwd")
 OPS = os.path.join(PKG, "_ops.so")
+OPS_TAG = os.path.join(PKG, "_build", "_ops.tag")  # what _ops.so was built against
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -100,10 +104,29 @@ def build_cli(force: bool = False) -> str:
     return CHPE_FWD
 
 
-def build_ops(force: bool = False) -> str:
+def _torch_tag() -> str:
+    """What _ops.so is built against: torch, Python; "" where torch, or its CUDA part, is missing."""
+    spec = importlib.util.find_spec("torch")
+    root = os.path.dirname(spec.origin) if spec and spec.origin else ""
+    if not root or not os.path.exists(os.path.join(root, "lib", "libc10_cuda.so")):
+        return ""
+    return f"{importlib.metadata.version('torch')} {sys.implementation.cache_tag} {root}"
+
+
+def build_ops(force: bool = False) -> str | None:
     """_ops.so, linked against the in-tree libchpe.so (found through $ORIGIN)
-    and the installed torch."""
-    if force or _stale(OPS, ["ops_torch.cpp", "../../include/chpe.h"]):
+    and the installed torch; None where there is none (the engine, its ctypes
+    interface and the command line do without)."""
+    tag = _torch_tag()
+    if not tag:
+        print("_ops.so is not built: no torch with CUDA", file=sys.stderr)
+        return None
+    try:
+        with open(OPS_TAG) as f:
+            same = f.read() == tag
+    except OSError:
+        same = False
+    if force or not same or _stale(OPS, ["ops_torch.cpp", "../../include/chpe.h"]):
         import sysconfig
 
         import torch
@@ -118,16 +141,15 @@ def build_ops(force: bool = False) -> str:
         cmd += ["-L", PKG, "-lchpe", "-Wl,-rpath,$ORIGIN", "-L", lib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
                 "-ltorch_python"]
         subprocess.run(cmd, check=True)
+        os.makedirs(os.path.dirname(OPS_TAG), exist_ok=True)
+        with open(OPS_TAG, "w") as f:
+            f.write(tag)
     return OPS
 
 
-def build_all(force: bool = False) -> None:
-    build_synth(force)
-    build_engine(force)
-    build_cli(force)
-    build_ops(force)
+def build_all(force: bool = False) -> list[str]:
+    return [p for p in (build_synth(force), build_engine(force), build_cli(force), build_ops(force)) if p]
 
 
 if __name__ == "__main__":
-    build_all(force="--force" in sys.argv)
-    print("built", LIBCHPE, LIBSYNTH)
+    print("built", *build_all(force="--force" in sys.argv))
