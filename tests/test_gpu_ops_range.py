@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 
 import chpe_qwen_engine_b200 as chpe
-from _ops_ref import attention
-from test_gpu_ops import DEV, check_paged, close, f64, i32, paged_case, put
+from _ops_ref import attention, logits
+from test_gpu_ops import DEV, check_paged, close, f64, i32, on_gpu, paged_case, put, rules_case
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -164,6 +164,37 @@ def test_paged_attention_infinite_keys_under_float_queries(cache):
     out = ops.attention_decode_paged(q, tk, tv, i32([[0]]), i32([5]), lse=lse)
     assert torch.isnan(out).all() and torch.isnan(lse).all()
     assert torch.equal(ops.attention_decode_paged(q, tk, tv, i32([[0]]), i32([2])), torch.ones_like(q))
+
+
+# ---- one long sequence among many short ones ----------------------------------------------
+@pytest.mark.parametrize("kind, H, KV, D", [("f16", 8, 2, 64), ("bf16", 16, 8, 128), ("f16", 8, 4, 256), ("bf16", 32, 2, 128)])
+@pytest.mark.parametrize("B, n", [(7, 20000), (32, 20000), (64, 20000), (200, 9000), (400, 9000)])
+def test_paged_attention_one_long_among_short(kind, H, KV, D, B, n):
+    """The long one is cut into far more records than the others."""
+    rng = np.random.default_rng(B)
+    page, each = 64, -(-n // 64)
+    lens = [10] * B
+    lens[B // 3] = n
+    table = np.full((B, each), -1, np.int32)
+    pages = rng.permutation(each + B)
+    table[B // 3] = pages[:each]
+    table[np.arange(B) != B // 3, 0] = pages[each:each + B - 1]
+    tk, xk = put(rng.standard_normal((each + B, page, KV, D)), kind)
+    tv, xv = put(rng.standard_normal((each + B, page, KV, D)), kind)
+    q, xq = put(rng.standard_normal((B, H, D)), kind)
+    check_paged(q, tk, tv, table, lens, xq, xk, xv, kind, kind, page)
+
+
+# ---- the largest tables of the logits rules ---------------------------------------------
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("B, V, L, n", [(1, 500003, 20000, 40000), (16, 300001, 17000, 33000), (1, 458752, 40000, 65535)])
+def test_logits_rules_largest_tables(kind, B, V, L, n):
+    """Counts of 32 bits, a bias place and a list entry for every token of a full slice, by 16 and by 8 CTAs per row."""
+    rng = np.random.default_rng(V)
+    x, x64, a = rules_case(rng, B, V, L, n, True, kind)
+    out, am = ops.logits_process(x, **on_gpu(a))
+    want, wam = logits(x64, **a, kind=np.float32)
+    assert np.array_equal(out.cpu().numpy(), want) and np.array_equal(am.cpu().numpy(), wam)
 
 
 # ---- buffers that overlap ------------------------------------------------------------
