@@ -43,7 +43,10 @@
 // lane).  P^T comes out of S^T by movmatrix.  Queries of the cache's type go in as
 // they are; float ones as two FP16 or three BF16 parts (22 and 24 bits), each a
 // column operand of its own, and so do the probabilities, held times 2^14 over
-// FP16, which keeps the small ones.  tcgen05.mma would need its operands in shared memory or TMEM in
+// FP16, which keeps the small ones.  A tile's products are summed from zero and then
+// added to the running sums in f32, because the instruction cuts what it adds to its
+// accumulator: over 131071 positions the output was off by 3.2e-6 of its norm, now by 4.5e-7
+// (f32 products by the library: 5.8e-7), for 93 us instead of 92.  tcgen05.mma would need its operands in shared memory or TMEM in
 // layouts of 128 rows for 8 columns of work; the tensor pipe is nearly idle either way.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -516,9 +519,13 @@ __global__ void __launch_bounds__(32 * Cfg<D, N>::kWarps) paged_kernel(const __g
           uint32_t vf[4];
           ldsm4t(vf, vb + v_row * C::kRow + (((2 * t + v_ch) ^ (v_row & 7)) << 4));
 #pragma unroll
-          for (int c = 0; c < N; c++)
+          for (int c = 0; c < N; c++) {
+            float add[4] = {};  // the smallest parts first
 #pragma unroll
-            for (int part = 0; part < PP; part++) mma16816<T>(o[c][t], vf, pb[c][part][0], pb[c][part][1]);
+            for (int part = PP - 1; part >= 0; part--) mma16816<T>(add, vf, pb[c][part][0], pb[c][part][1]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[c][t][e] += add[e];
+          }
         }
       }
       __syncwarp();  // the stage may be filled again

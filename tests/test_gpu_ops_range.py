@@ -44,6 +44,25 @@ def test_probabilities_keep_f32_bits_over_a_bf16_cache(kind, D):
     close(out, ref, e * (2 * p / (2 + p))[None, :, None], kind)
 
 
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("KV, D", [(8, 64), (8, 128), (4, 256)])
+def test_sums_over_positions_are_rounded_not_cut(cache, KV, D):
+    """All weights 1, the first value 16, then every 16 positions three quarters of a step of
+    the sum: cut, none of them would count."""
+    m, B, page = 40, 300, 16
+    k = np.zeros((m, page, KV, D))
+    v = np.zeros((m, page, KV, D))
+    v[0, 0], v[1:, 0] = 16.0, 0.75 * 2.0 ** -19
+    tk, tv = put(k, cache)[0], put(v, cache)[0]
+    q = torch.zeros(B, KV, D, device=DEV)
+    n = page * m
+    out = ops.attention_decode_paged(q, tk, tv, i32(np.arange(m)[None]).expand(B, -1), i32([n] * B))
+    ref = (16.0 + (m - 1) * 0.75 * 2.0 ** -19) / n * np.ones((B, KV, D))
+    # an addition for every 16 positions, each off by half a step (2^-24 of the sum); the joins
+    # of a few records, the quotient and its product
+    close(out, ref, ref * (m - 1 + 8) * 2.0 ** -24, "f32")
+
+
 def test_the_longest_batch_repeats_its_bits():
     g = torch.Generator(DEV).manual_seed(5)
     n, page = 131071, 64
