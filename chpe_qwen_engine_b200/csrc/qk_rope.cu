@@ -129,9 +129,9 @@ CHPE_DEV void store8<__nv_bfloat16>(__nv_bfloat16* p, const float (&x)[8]) {
 CHPE_DEV float2 cos_sin_turn(uint64_t f) {
   const uint64_t up = f + (1ull << 61);             // + 1/8 turn
   const uint32_t quad = (uint32_t)(up >> 62);       // nearest quarter turn
-  const int32_t r = (int32_t)((uint32_t)(up >> 30) ^ 0x80000000u);  // [-1/8, 1/8) turn in units of 2^-34
+  const int64_t r = (int64_t)(up & ((1ull << 62) - 1)) - (1ll << 61);  // [-1/8, 1/8) turn
   float s, c;
-  sincospif((float)r * 0x1p-33f, &s, &c);  // half turns
+  sincospif((float)r * 0x1p-63f, &s, &c);  // half turns
   const float cc = (quad & 1u) ? s : c, ss = (quad & 1u) ? c : s;
   return make_float2((quad == 1u || quad == 2u) ? -cc : cc, quad >= 2u ? -ss : ss);
 }

@@ -185,6 +185,24 @@ def test_paged_attention_infinite_keys_under_float_queries(cache):
     assert torch.equal(ops.attention_decode_paged(q, tk, tv, i32([[0]]), i32([2])), torch.ones_like(q))
 
 
+# ---- angles ----------------------------------------------------------------------------
+@pytest.mark.parametrize("theta", [1e4, 1e7])
+def test_angles_of_every_size_keep_f32_bits(theta):
+    """Pairs (1, 0) turn into the cosine and the sine, each right to its own last bits, those
+    of an angle of 1e-7 too."""
+    pos = np.array([1, 2, 7, 1000, 131071, 2 ** 30 + 1, -5])
+    f = ops.rope_inv_freq(theta, 128)
+    x = torch.zeros(len(pos), 1, 128, device=DEV)
+    x[..., :64] = 1.0
+    out, _ = ops.qk_norm_rope(x, x, None, i32(pos), f)
+    a = pos[:, None].astype(np.longdouble) * f.astype(np.longdouble)
+    for got, ref in ((out[:, 0, :64], np.cos(a)), (out[:, 0, 64:], np.sin(a))):
+        # the angle's rounding and sincospi's 2 ulp of the result; the fixed point's 2^-65 turn of a
+        # position, and the reference's 2^-63 of the angle
+        tol = (1 + 4) * 2.0 ** -24 * np.abs(ref) + np.abs(pos)[:, None] * 2.0 ** -61
+        assert np.all(np.abs(f64(got) - ref) <= tol)
+
+
 # ---- one long sequence among many short ones ----------------------------------------------
 @pytest.mark.parametrize("kind, H, KV, D", [("f16", 8, 2, 64), ("bf16", 16, 8, 128), ("f16", 8, 4, 256), ("bf16", 32, 2, 128)])
 @pytest.mark.parametrize("B, n", [(7, 20000), (32, 20000), (64, 20000), (200, 9000), (400, 9000)])
