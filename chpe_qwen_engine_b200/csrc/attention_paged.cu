@@ -28,9 +28,9 @@
 // ahead across the ends of sequences, a running maximum and sums in registers, and
 // waits for no other warp; only warps that share a head meet, at the end of a part.
 //
-// Measured (device time): 131071 positions of one sequence on 64/8 heads of 128: 92 us,
-// 91 % of the copy rate; 64 sequences of up to 8192 there: 122 us, 92 %; 37 of up
-// to 4093 on 16/4 heads of 256: 43 us, 76 %; one of 77 on 16/2 heads: 7.9 us.
+// Measured (device time, replayed from a graph): 131071 positions of one sequence on 64/8
+// heads of 128 in BF16: 93 us, 89 % of the copy rate; 64 sequences of up to 8192 there: 122 us, 92 %, with
+// float queries 120; 37 of up to 4093 on 16/4 heads of 256: 43.5 us, 75 %; one of 77 on 16/2 heads: 8 us.
 // What is left: SMs get bandwidth unevenly, so that CTAs with equal shares end
 // 10 % before and after the mean, and the records' join, 3 us behind a gap of 2.
 // Handing a fifth of the line out to whoever is done evened the ends out but cost as
@@ -47,7 +47,7 @@
 // added to the running sums in f32, because the instruction cuts what it adds to its
 // accumulator: over 131071 positions the output was off by 3.2e-6 of its norm, now by 4.5e-7
 // (f32 products by the library: 5.8e-7), for 93 us instead of 92.  tcgen05.mma would need its operands in shared memory or TMEM in
-// layouts of 128 rows for 8 columns of work; the tensor pipe is nearly idle either way.
+// layouts of 128 rows for 8 columns of work; the tensor pipe is busy 14 to 19 % of the time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -815,11 +815,14 @@ cudaError_t launch(PagedLaunch P, void* workspace, int device, cudaStream_t s) {
   const cudaError_t e = cudaLaunchKernelEx(&main.cfg, paged_kernel<T, TQ, D, N>, P);
   if (e != cudaSuccess) return e;
   const int cuts = P.by_seq ? P.B * P.groups : grid;
-  // The records that a group may be cut into.  Many: 16 warps for 64 values of a query
-  // head (two sequences of 2048 on 64/8 heads, 76 records each: 10.5 us, with four warps
-  // per head 11.3, with one 17.1).  Some: four warps per query head (eight sequences,
-  // 20 records: 22.1 us, with 16 warps 28.6, with one 23.7).  Few: one warp each (64
-  // sequences of up to 1024, two or three records: 31.3 us, with four warps 34.9).
+  // The records that a group of an even batch is cut into; which kernel joins them goes by
+  // that, and each joins any number.  Many: 16 warps for 64 values of a query head (two
+  // sequences of 2048 on 64/8 heads, 76 records each: 10.6 us, with four warps per head
+  // 10.8, with one 16.8).  Some: four warps per query head (eight sequences, 20 records:
+  // 21.0 us, with 16 warps 27.3, with one 21.7).  Few: one warp each (64 sequences of up to
+  // 1024, two or three records: 25.8 us, with four warps 29.0, with 16 66.2).  An uneven
+  // batch pays for the estimate: one sequence of 131071 among 63 of ten, some 140 records,
+  // takes 104 us where four warps per head take 98.
   const int64_t records = (P.cap >> P.tile_shift) < grid / cuts + 2 ? (P.cap >> P.tile_shift) : grid / cuts + 2;
   if (records > 64) {
     chpe::ServeLaunch join(dim3(cuts, P.HW * C::kWarpHeads * (D / 64)), 32 * 16, 0, s);
@@ -922,8 +925,8 @@ extern "C" int chpe_attention_decode_paged(const void* q, int dtype, int64_t q_s
   P.G = P.H / P.KV;
   // More than 8 query heads per kv head: two operands per warp, so that the rows copied
   // serve 16, or two warps that copy the same rows.  At heads of 128 the former takes 72
-  // instead of 82 us for 64 sequences of up to 8192 on 64/4 heads, but 11.4 instead of
-  // 9.8 for one of 4000 on 32/2, so it is taken where the tables have room for 64 MB of
+  // instead of 86 us for 64 sequences of up to 8192 on 64/4 heads in BF16, but 11.1 instead
+  // of 9.8 for one of 4000 on 32/2, so it is taken where the tables have room for 64 MB of
   // entries; at 64 they are even (26.9 us), and at 256 the registers are lacking.
   const double room = 4.0 * batch * P.cap * num_kv_heads * head_dim;
   const int operands = head_dim == 128 && P.G > kHeads && room >= 64.0 * (1 << 20) ? 2 : 1;

@@ -332,11 +332,12 @@ int chpe_attention_decode_noalloc(const float *q, const float *k, const float *v
  * sampling rules.  They share one manner:
  *
  * Types: CHPE_F32, CHPE_F16, CHPE_BF16 below.  Strides count elements; a
- * stride is not looked at where there is one row.  All arithmetic is f32 with
- * one rounding at the store.
+ * stride is not looked at where there is one row.  Values are f32 from the load
+ * to one rounding at the store, sums are f32; what is held in less is named with
+ * the operator.
  * Cache: K and V of one layer, each [num_pages][page_size][num_kv_heads]
- * [head_dim] of FP16 or BF16, the layout of the engine's own pools; a slot is
- * the row page * page_size + offset.  head_dim is 64, 128 or 256.
+ * [head_dim] of FP16 or BF16; a slot is the row page * page_size + offset.
+ * head_dim is 64, 128 or 256.
  * Calls are asynchronous on `stream` (a cudaStream_t of the buffers' device;
  * NULL: its default stream), allocate nothing, read nothing back and can be
  * captured into a graph.  The buffers lie on one device, which need not be
@@ -360,7 +361,8 @@ int chpe_attention_decode_noalloc(const float *q, const float *k, const float *v
  * positions[t] * inv_freq[i], i < rope_dim/2 (rotate-half; dimensions from
  * rope_dim on stay), rope_dim a multiple of 16 up to head_dim, 0: none.
  * inv_freq is a HOST array of rope_dim/2 doubles within +-16, copied by the call;
- * angles are exact for every int32 position.
+ * the angle is held to 2^-65 of a turn per position until it is rounded to f32, and the
+ * norm's root is within 2 ulp.
  * q [num_tokens][num_heads][head_dim], k and v [num_tokens][num_kv_heads]
  * [head_dim], heads contiguous, tokens q_stride / k_stride / v_stride elements
  * apart (one buffer may hold all three).  q_out gets the queries; k_out (or
@@ -400,8 +402,11 @@ int chpe_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, in
  * parts (unless no part is 0 and all have one sign).  A value that is infinite or
  * NaN makes its dimension infinite or NaN for the query heads of its kv head, at
  * weight 0 too; lse is not touched.
- * The cache has q's type, or any when q is float.  Results do not depend on
- * timing: the same call gives the same bits.
+ * The cache has q's type, or any when q is float.  Products are of the cache's
+ * type with f32 sums: float queries and the softmax's weights enter as sums of
+ * parts, with 22 bits over FP16 (a query's value below 2^-16 of its head's
+ * largest with an error of 2^-39 of that) and 24 over BF16.  Results do not depend
+ * on timing: the same call gives the same bits.
  * workspace: chpe_attention_decode_paged_workspace(head_dim) bytes (0 for an
  * unsupported head_dim), 16-byte aligned, of any content; calls that may
  * overlap on the GPU need one each. */

@@ -39,9 +39,10 @@ def attention(q, kc, vc, table, lens, scale, page, kind, cache_kind):
     G = H // KV
     out, lse = np.zeros((B, H, D)), np.full((B, H), -np.inf)
     b_out, b_lse = np.zeros((B, H, D)), np.zeros((B, H))
-    # products carry q in two or four parts: FP16 22 bits, BF16 16 (exact for BF16 queries) or 32
+    # queries of the cache's type go into the products as they are, float ones in two FP16 parts
+    # (22 bits) or three BF16 parts (24)
     q_part = {"f16": 2.0 ** -22, "bf16": 0.0}[cache_kind] + 2.0 ** -24
-    # the probability in two parts (four for float queries over BF16)
+    # and so do the probabilities of all of them (the bound allows BF16 queries 16 bits)
     p_part = 2.0 ** -22 if cache_kind == "f16" else 2.0 ** -17 if kind != "f32" else 2.0 ** -24
     for b in range(B):
         n = int(min(max(lens[b], 0), table.shape[1] * page))
