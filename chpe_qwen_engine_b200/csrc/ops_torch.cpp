@@ -56,6 +56,12 @@ int dtype_of(const Tensor& t, const char* name) {
   }
 }
 
+// The operators have no gradient: one that autograd would expect must not get lost.
+void no_gradient(const Tensor& t, const char* name) {
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    unfit(std::string(name) + " requires a gradient, which this operator does not have: call it under torch.no_grad()");
+}
+
 // ---- arguments: positional and by name -----------------------------------------
 template <int N>
 struct Args {
@@ -89,9 +95,7 @@ struct Args {
     }
     if (!THPVariable_Check(at[i])) throw Misuse(std::string(name) + " must be a tensor");
     const Tensor& t = THPVariable_Unpack(at[i]);
-    // the operators have no gradient: one that autograd would expect must not get lost
-    if (t.requires_grad() && c10::GradMode::is_enabled())
-      throw Unfit(std::string(name) + " requires a gradient, which this operator does not have: call it under torch.no_grad()");
+    no_gradient(t, name);
     return &t;
   }
   double number(int i, const char* name, double def) const {
@@ -221,6 +225,7 @@ struct Frequencies {
     if (!o) return;
     if (THPVariable_Check(o)) {
       const Tensor& t = THPVariable_Unpack(o);
+      no_gradient(t, "inv_freq");
       want(t.is_cpu() && t.scalar_type() == at::kDouble && t.dim() == 1 && t.is_contiguous(), what);
       data = static_cast<const double*>(t.data_ptr());
       n = t.size(0);

@@ -330,6 +330,7 @@ def test_gradients_are_refused_and_no_grad_is_not():
     one = torch.ones(2, device=DEV)
     calls = [("q_weight", lambda: ops.qk_norm_rope(q, q, None, pos, freq, q_weight=w)),
              ("k", lambda: ops.qk_norm_rope(q, p(q.clone()), None, pos, freq)),
+             ("inv_freq", lambda: ops.qk_norm_rope(q, q, None, pos, p(torch.from_numpy(freq)))),
              ("q", lambda: ops.attention_decode_paged(p(q.clone()), kc, kc, table, lens)),
              ("v_cache", lambda: ops.attention_decode_paged(q, kc, p(kc.clone()), table, lens)),
              ("out", lambda: ops.attention_decode_paged(q, kc, kc, table, lens, out=p(q.clone()))),
